@@ -71,6 +71,14 @@ SIGNATURES = {
     "jllm_hip_softmax_inplace": (I, [P, I, P]),
     "jllm_hip_gemv_dense": (I, [P, P, I, P, I, I, P]),
     "jllm_hip_gemm_dense_batched": (I, [P, P, I, P, I, I, I, P]),
+    # batched serving over a paged KV cache
+    "jllm_hip_qk_norm_rope_store_kv_paged": (I, [P, I64, P, I64, P, I64, P, I64, P, P, I, F, P, P, P, P, I64, P, P,
+                                                 I, I, I, I, I, F, I, I, P]),
+    "jllm_hip_flash_attention_decode_paged_workspace": (I64, [I, I, I, I, I, I]),
+    "jllm_hip_flash_attention_decode_paged": (I, [P, P, I64, P, P, P, P, I, I, P, I64, P, I, I, I, I, I, I, F, I, I,
+                                                  P, I64, P]),
+    "jllm_hip_logits_process_workspace": (I64, [I, I]),
+    "jllm_hip_logits_process": (I, [P, I64, P, I64, I, I, P, I64, P, P, P, P, P, P, P, I64, P, P, I64, P, P, I64, P]),
     # GGUF reader / loader / writer
     "jllm_hip_gguf_open": (P, [ctypes.c_char_p]),
     "jllm_hip_gguf_close": (None, [P]),

@@ -402,6 +402,97 @@ int jllm_hip_gemv_dense(uint16_t* out, const void* W, int wtype, const uint16_t*
 int jllm_hip_gemm_dense_batched(uint16_t* out, const void* W, int wtype, const uint16_t* x, int M, int N, int K,
                                 void* stream);
 
+/* ---- batched serving: several sequences over one paged KV cache ----
+ * (no reference counterpart: the engine serves one sequence over one
+ * contiguous cache.)
+ *
+ * A page pool is k_pages / v_pages [n_pages][page_size][n_kv_heads][cache_head_dim]
+ * (int8 or fp16) and, for INT8, k_scales / v_scales fp32
+ * [n_pages][page_size][n_kv_heads]; slot s is row s % page_size of page
+ * s / page_size.  Position t of a sequence lies in the page
+ * block_table[row][t / page_size], at t % page_size.  Lengths, positions,
+ * slots and page ids are int32 in device memory, read when the kernels run
+ * (a captured graph serves every step) and checked there: nothing outside
+ * the pool is read or written, whatever they hold.  These calls keep no
+ * state and use no library-owned scratch: calls on different streams, or
+ * graphs that may run at once, need workspaces of their own and are
+ * otherwise independent. */
+
+/* The attention front of N tokens of any sequences, in one launch: RMSNorm
+ * over each head of q and k (both weights given, or both NULL), RoPE of q and
+ * k at positions[t], q to q_out, k and v into slot slots[t] of the pool: fp16,
+ * or int8 codes rint(v * 127 / absmax) with the scale absmax / 127 of each
+ * (slot, head).  Everything is computed in fp32 from the fp16 inputs and
+ * rounded once, where it is stored; the angle is exact to 2^-32 turns at
+ * every position (jllm_hip_qk_norm_rope_store_kv keeps the reference's
+ * intermediate roundings and fp32 angle).  An int8 row that holds a NaN or an
+ * infinity gets a NaN scale.
+ * q_out, q, k, v: rows of q_out_stride, q_stride, ... halves (multiples of
+ * 4: slices of a fused QKV buffer will do), 8-byte aligned; q_out may be q.
+ * A token whose slot is outside [0, n_slots) is padding: its q_out row and
+ * the pool are left as they are.  The slots of one call must be distinct.
+ * head_dim a multiple of 8 up to 128; pages 16-byte aligned, cache rows a
+ * multiple of 16 bytes.  neox and norm_fp32 as jllm_hip_qk_norm_rope_store_kv. */
+int jllm_hip_qk_norm_rope_store_kv_paged(uint16_t* q_out, int64_t q_out_stride, const uint16_t* q, int64_t q_stride,
+                                         const uint16_t* k, int64_t k_stride, const uint16_t* v, int64_t v_stride,
+                                         const void* q_norm, const void* k_norm, int norm_fp32, float eps,
+                                         void* k_pages, void* v_pages, float* k_scales, float* v_scales,
+                                         int64_t n_slots, const int32_t* positions, const int32_t* slots,
+                                         int n_heads, int n_kv_heads, int head_dim, int cache_head_dim, int N,
+                                         float theta_base, int neox, int kv_int8, void* stream);
+
+/* Decode attention of B query rows, each over its own sequence: row b
+ * attends to positions [0, seq_lens[b]) (the last `window` of them when
+ * window > 0) of block_table row b, i.e. block_table + b * table_stride.
+ * q rows of q_stride halves (a multiple of 8), out [B][n_heads * head_dim]
+ * fp16.  A row of length <= 0 gives zeros; a length above max_seq counts as
+ * max_seq (host: the longest a row can be; it sizes the split of the keys).
+ * The keys of a page id outside [0, n_pages) are skipped.  Slots of a page
+ * behind the end of its sequence may hold anything.  Several query tokens
+ * of one sequence (a prompt chunk) are passed as one row each, with the same
+ * table row and growing lengths.
+ * page_size a power of two from 16 to 4096; head_dim, heads and KV types
+ * as in jllm_hip_flash_attention_decode, n_heads <= 4096 (scales NULL = 1.0).
+ * workspace: 16-byte aligned, any content, at least the bytes that
+ * jllm_hip_flash_attention_decode_paged_workspace says, which returns a
+ * negative JLLM_ERR_* for sizes that the operator refuses. */
+int64_t jllm_hip_flash_attention_decode_paged_workspace(int B, int n_heads, int n_kv_heads, int head_dim, int max_seq,
+                                                        int window);
+int jllm_hip_flash_attention_decode_paged(uint16_t* out, const uint16_t* q, int64_t q_stride, const void* k_pages,
+                                          const void* v_pages, const float* k_scales, const float* v_scales,
+                                          int n_pages, int page_size, const int32_t* block_table,
+                                          int64_t table_stride, const int32_t* seq_lens, int B, int n_heads,
+                                          int n_kv_heads, int head_dim, int cache_head_dim, int max_seq, float scale,
+                                          int kv_int8, int window, void* workspace, int64_t workspace_bytes,
+                                          void* stream);
+
+/* Penalties, biases and grammar masks on the fp32 logits [B][V] (rows of
+ * logits_stride floats) of a batch, to out (rows of out_stride floats; may be
+ * logits itself), and each row's greedy token.  Per row b, in this order:
+ *   y = x > 0 ? x / repetition[b] : x * repetition[b]  for every token among
+ *       the first n_tokens[b] of tokens + b * token_stride,
+ *   y = y - frequency[b] * count, then y = y - presence[b], for those that
+ *       occur count > 0 times behind the first n_prompt[b] (the output),
+ *   y = y + bias for the first n_bias[b] of bias_ids + b * bias_stride (of a
+ *       token that is listed twice the last entry counts),
+ *   y = -inf for tokens whose bit (token % 32 of word token / 32) of
+ *       mask + b * mask_stride is 0.
+ * tokens, bias_ids, mask and next_token may be NULL (that part is skipped),
+ * as may n_prompt (0), repetition (1), frequency and presence (0).  Counts
+ * are held to [0, stride], n_prompt to [0, n_tokens]; ids outside [0, V) are
+ * ignored.  next_token[b] = the lowest index of the largest finite y, -1 when
+ * none is finite (a mask that leaves nothing); jllm_hip_dequant_embedding_rows
+ * reads -1 as a zero row.
+ * workspace (for next_token only): 8-byte aligned, at least the bytes that
+ * jllm_hip_logits_process_workspace says. */
+int64_t jllm_hip_logits_process_workspace(int B, int V);
+int jllm_hip_logits_process(float* out, int64_t out_stride, const float* logits, int64_t logits_stride, int B, int V,
+                            const int32_t* tokens, int64_t token_stride, const int32_t* n_prompt,
+                            const int32_t* n_tokens, const float* repetition, const float* frequency,
+                            const float* presence, const int32_t* bias_ids, const float* bias, int64_t bias_stride,
+                            const int32_t* n_bias, const uint32_t* mask, int64_t mask_stride, int32_t* next_token,
+                            void* workspace, int64_t workspace_bytes, void* stream);
+
 /* ---- decoder loop (the engine-side caller of the kernels above) ---- */
 
 /* Model shape (ModelConfig, include/jllm_engine.h:59; Llama/Qwen3 family: RMSNorm,
