@@ -28,10 +28,11 @@ def _sources():
     return sorted(f for f in os.listdir(CSRC) if f.endswith((".hip", ".cpp")))
 
 
-# per-source flags: the MMQ kernels keep their matrix-core results in VGPRs
-# (the fp32 epilogue reads every result element; AGPR results would cost one
-# v_accvgpr_read per element)
-FILE_FLAGS = {"mmq.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+# per-source flags: the MMQ and paged attention kernels keep their matrix-core
+# results in VGPRs (the fp32 epilogue reads, and the softmax rescales, every
+# result element; AGPR results would cost one v_accvgpr_read per element)
+FILE_FLAGS = {"mmq.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+              "paged_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 
 
 def _compile(src):
