@@ -13,50 +13,92 @@
 namespace jllm_hip {
 
 constexpr int LG_THREADS = 256;
-constexpr int LG_CHUNK = 4096;                 // tokens a workgroup takes
 constexpr uint32_t LG_PROMPT = 0x80000000u;    // "in the prompt" bit of a count
 
+// rows begin at any 4-byte address
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef int32_t i32x4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u32x4l __attribute__((ext_vector_type(4)));
 
 // (value, index) as one word that grows with the value and falls with the index;
-// 0 for what the pick ignores
+// 0: nothing to pick
 __device__ __forceinline__ uint64_t pick_key(float y, int i) {
-    if (!isfinite(y)) return 0;
     const uint32_t b = __builtin_bit_cast(uint32_t, y + 0.0f);      // -0 counts as +0
     const uint32_t o = b & 0x80000000u ? ~b : b | 0x80000000u;
     return ((uint64_t)o << 32) | (uint32_t)~i;
 }
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_umax(uint32_t v) {
+    return max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xF, 0xF, false));
+}
+__device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
+    v = dpp_umax<0xB1>(v);
+    v = dpp_umax<0x4E>(v);
+    v = dpp_umax<0x141>(v);
+    v = dpp_umax<0x140>(v);
+    const uint32_t a = max((uint32_t)__builtin_amdgcn_readlane((int)v, 0), (uint32_t)__builtin_amdgcn_readlane((int)v, 16));
+    const uint32_t b = max((uint32_t)__builtin_amdgcn_readlane((int)v, 32), (uint32_t)__builtin_amdgcn_readlane((int)v, 48));
+    return max(a, b);
+}
 __device__ __forceinline__ uint64_t wave_max_key(uint64_t k) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const uint64_t v = __shfl_xor((unsigned long long)k, o, 64);
-        k = v > k ? v : k;
-    }
-    return k;
+    const uint32_t hi = wave_umax((uint32_t)(k >> 32));
+    const uint32_t lo = wave_umax((uint32_t)(k >> 32) == hi ? (uint32_t)k : 0u);
+    return ((uint64_t)hi << 32) | lo;
 }
 
+// A workgroup takes CH = 1024 J tokens of a row, a thread J times four neighbours.
+// The logits and mask words are on their way while the lists are searched: every
+// workgroup goes through its row's whole lists and counts the tokens that fall
+// into its part in LDS (integers: the order of the atomics does not matter).
+template <int J>
 __global__ __launch_bounds__(LG_THREADS) void logits_kernel(LogitsArgs a) {
 #pragma clang fp contract(off)
-    __shared__ uint32_t sCount[LG_CHUNK];
-    __shared__ uint32_t sBias[LG_CHUNK];
+    constexpr int CH = 1024 * J;
+    extern __shared__ __attribute__((aligned(16))) uint32_t sLists[];
     __shared__ uint64_t sKey[LG_THREADS / 64];
+    uint32_t* sCount = sLists;                             // [CH] when there are tokens
+    uint32_t* sBias = sLists + (a.tokens ? CH : 0);        // [CH] when there are biases: entry + 1
     const int64_t b = blockIdx.y;
-    const int t = threadIdx.x, c0 = blockIdx.x * LG_CHUNK, n = min(LG_CHUNK, a.V - c0);
-    if (a.tokens) for (int i = t; i < LG_CHUNK; i += LG_THREADS) sCount[i] = 0;
-    if (a.bias_ids) for (int i = t; i < LG_CHUNK; i += LG_THREADS) sBias[i] = 0;
-    __syncthreads();
+    const int t = threadIdx.x, c0 = blockIdx.x * CH, n = min(CH, a.V - c0);
+    const float* x = a.x + b * a.x_stride + c0;
+    float* out = a.out + b * a.out_stride + c0;
+
+    f32x4u y[J];
+    uint32_t word[J];
+#pragma unroll
+    for (int j = 0; j < J; j++) {
+        const int i = 1024 * j + 4 * t;
+        if (i + 4 <= n) y[j] = *(const f32x4u*)(x + i);
+        else
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[j][e] = i + e < n ? x[i + e] : 0.0f;
+        word[j] = a.mask && i < n ? a.mask[b * a.mask_stride + ((c0 + i) >> 5)] : ~0u;
+    }
+    __builtin_amdgcn_sched_barrier(0);
+
+    const int lists = (a.tokens ? CH : 0) + (a.bias_ids ? CH : 0);
+    if (lists) {
+        for (int i = 4 * t; i < lists; i += 4 * LG_THREADS) *(u32x4l*)(sLists + i) = u32x4l{0u, 0u, 0u, 0u};
+        __syncthreads();
+    }
     if (a.tokens) {
         const int nt = (int)max((int64_t)0, min((int64_t)a.n_tokens[b], a.token_stride));
         const int np = a.n_prompt ? max(0, min(a.n_prompt[b], nt)) : 0;
         const int32_t* ids = a.tokens + b * a.token_stride;
-        for (int i = t; i < nt; i += LG_THREADS) {
-            const uint32_t at = (uint32_t)ids[i] - (uint32_t)c0;
+        auto count = [&](int id, int i) {
+            const uint32_t at = (uint32_t)id - (uint32_t)c0;
             if (at < (uint32_t)n) {
                 if (i < np) atomicOr(&sCount[at], LG_PROMPT);
                 else atomicAdd(&sCount[at], 1u);
             }
+        };
+        const int n4 = nt & ~3;
+        for (int i = 4 * t; i < n4; i += 4 * LG_THREADS) {
+            const i32x4u v = *(const i32x4u*)(ids + i);
+#pragma unroll
+            for (int e = 0; e < 4; e++) count(v[e], i + e);
         }
+        if (n4 + t < nt) count(ids[n4 + t], n4 + t);
     }
     if (a.bias_ids) {
         const int nb = (int)max((int64_t)0, min((int64_t)a.n_bias[b], a.bias_stride));
@@ -66,68 +108,92 @@ __global__ __launch_bounds__(LG_THREADS) void logits_kernel(LogitsArgs a) {
             if (at < (uint32_t)n) atomicMax(&sBias[at], (uint32_t)i + 1u);
         }
     }
-    __syncthreads();
-    const float rep = a.repetition ? a.repetition[b] : 1.0f;
-    const float freq = a.frequency ? a.frequency[b] : 0.0f, pres = a.presence ? a.presence[b] : 0.0f;
-    const float* x = a.x + b * a.x_stride + c0;
-    float* out = a.out + b * a.out_stride + c0;
-    uint64_t best = 0;
-    for (int i = t; i < n; i += LG_THREADS) {
-        float y = x[i];
+    if (lists) __syncthreads();
+    const float rep = a.tokens && a.repetition ? a.repetition[b] : 1.0f;
+    const float freq = a.tokens && a.frequency ? a.frequency[b] : 0.0f;
+    const float pres = a.tokens && a.presence ? a.presence[b] : 0.0f;
+    float best = -INFINITY;
+    int at = -1;
+#pragma unroll
+    for (int j = 0; j < J; j++) {
+        const int i = 1024 * j + 4 * t;
         if (a.tokens) {
-            const uint32_t c = sCount[i];
-            if (c) {
-                y = y > 0.0f ? y / rep : y * rep;
-                const uint32_t cnt = c & ~LG_PROMPT;
-                if (cnt) { y = y - freq * (float)cnt; y = y - pres; }
+            const u32x4l c4 = *(const u32x4l*)(sCount + i);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if (c4[e]) {
+                    y[j][e] = y[j][e] > 0.0f ? y[j][e] / rep : y[j][e] * rep;
+                    const uint32_t cnt = c4[e] & ~LG_PROMPT;
+                    if (cnt) { y[j][e] = y[j][e] - freq * (float)cnt; y[j][e] = y[j][e] - pres; }
+                }
             }
         }
         if (a.bias_ids) {
-            const uint32_t j = sBias[i];
-            if (j) y = y + a.bias[b * a.bias_stride + j - 1];
+            const u32x4l c4 = *(const u32x4l*)(sBias + i);
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (c4[e]) y[j][e] = y[j][e] + a.bias[b * a.bias_stride + c4[e] - 1];
         }
-        if (a.mask && !((a.mask[b * a.mask_stride + ((c0 + i) >> 5)] >> (i & 31)) & 1u)) y = -INFINITY;
-        out[i] = y;
-        const uint64_t k = pick_key(y, c0 + i);
-        best = k > best ? k : best;
+        const uint32_t bits = word[j] >> (i & 31);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            if (!(bits >> e & 1u)) y[j][e] = -INFINITY;
+            if (i + e < n && fabsf(y[j][e]) < INFINITY && (at < 0 || y[j][e] > best)) { best = y[j][e]; at = i + e; }
+        }
+        if (i + 4 <= n) *(f32x4u*)(out + i) = y[j];
+        else
+#pragma unroll
+            for (int e = 0; e < 4; e++) if (i + e < n) out[i + e] = y[j][e];
     }
     if (!a.next_token) return;
-    best = wave_max_key(best);
-    if ((t & 63) == 0) sKey[t >> 6] = best;
+    uint64_t key = wave_max_key(at >= 0 ? pick_key(best, c0 + at) : 0);
+    if ((t & 63) == 0) sKey[t >> 6] = key;
     __syncthreads();
     if (t == 0) {
-        for (int w = 1; w < LG_THREADS / 64; w++) best = sKey[w] > best ? sKey[w] : best;
-        if (gridDim.x == 1) a.next_token[b] = best ? (int32_t)~(uint32_t)best : -1;
-        else a.cand[b * gridDim.x + blockIdx.x] = best;
+#pragma unroll
+        for (int w = 1; w < LG_THREADS / 64; w++) key = max(key, sKey[w]);
+        if (gridDim.x == 1) a.next_token[b] = key ? (int32_t)~(uint32_t)key : -1;
+        else a.cand[b * gridDim.x + blockIdx.x] = key;
     }
 }
 
-__global__ __launch_bounds__(64) void logits_pick_kernel(int32_t* tok, const uint64_t* cand, int chunks) {
-    const int64_t b = blockIdx.x;
-    uint64_t best = 0;
-    for (int i = threadIdx.x; i < chunks; i += 64) {
-        const uint64_t k = cand[b * chunks + i];
-        best = k > best ? k : best;
-    }
-    best = wave_max_key(best);
-    if (threadIdx.x == 0) tok[b] = best ? (int32_t)~(uint32_t)best : -1;
+// one wave per row
+__global__ __launch_bounds__(LG_THREADS) void logits_pick_kernel(int32_t* tok, const uint64_t* cand, int chunks, int B) {
+    const int64_t b = (int64_t)blockIdx.x * (LG_THREADS / 64) + (threadIdx.x >> 6);
+    const int l = threadIdx.x & 63;
+    if (b >= B) return;
+    uint64_t key = 0;
+#pragma unroll 4
+    for (int i = l; i < chunks; i += 64) key = max(key, cand[b * chunks + i]);
+    key = wave_max_key(key);
+    if (l == 0) tok[b] = key ? (int32_t)~(uint32_t)key : -1;
 }
 
 namespace {
-int logits_chunks(int V) { return (int)(((int64_t)V + LG_CHUNK - 1) / LG_CHUNK); }
+// Few rows: short parts, so that the row is spread over the card; many rows: long
+// parts, which search the lists less often.
+int logits_part(int B, int V) { return (int64_t)B * ((V + 4095) / 4096) < 512 ? 1 : 4; }
+int logits_chunks(int B, int V) {
+    const int ch = 1024 * logits_part(B, V);
+    return (int)(((int64_t)V + ch - 1) / ch);
+}
 }  // namespace
 
 int64_t logits_workspace(int B, int V) {
-    const int n = logits_chunks(V);
+    const int n = logits_chunks(B, V);
     return n > 1 ? (int64_t)B * n * 8 : 0;
 }
 
 hipError_t logits_launch(const LogitsArgs& a, hipStream_t st) {
-    const int n = logits_chunks(a.V);
-    hipLaunchKernelGGL(logits_kernel, dim3(n, a.B), dim3(LG_THREADS), 0, st, a);
+    const int n = logits_chunks(a.B, a.V), J = logits_part(a.B, a.V);
+    const dim3 grid(n, a.B);
+    const size_t lds = (size_t)((a.tokens ? 1 : 0) + (a.bias_ids ? 1 : 0)) * J * 4096;
+    if (J == 1) hipLaunchKernelGGL((logits_kernel<1>), grid, dim3(LG_THREADS), lds, st, a);
+    else        hipLaunchKernelGGL((logits_kernel<4>), grid, dim3(LG_THREADS), lds, st, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !a.next_token || n == 1) return e;
-    hipLaunchKernelGGL(logits_pick_kernel, dim3(a.B), dim3(64), 0, st, a.next_token, (const uint64_t*)a.cand, n);
+    hipLaunchKernelGGL(logits_pick_kernel, dim3((a.B + 3) / 4), dim3(LG_THREADS), 0, st, a.next_token,
+                       (const uint64_t*)a.cand, n, a.B);
     return hipGetLastError();
 }
 

@@ -52,135 +52,223 @@ __device__ __forceinline__ uint32_t group_max_dpp(uint32_t v) {
 }
 
 __device__ __forceinline__ u32x2f pack4(const float* x) {
-    return u32x2f{(uint32_t)f32_to_f16_bits(x[0]) | ((uint32_t)f32_to_f16_bits(x[1]) << 16),
-                  (uint32_t)f32_to_f16_bits(x[2]) | ((uint32_t)f32_to_f16_bits(x[3]) << 16)};
+    return u32x2f{h2_bits(half2_t{(_Float16)x[0], (_Float16)x[1]}), h2_bits(half2_t{(_Float16)x[2], (_Float16)x[3]})};
 }
+// the codes rint(x * inv): x * inv + 1.5 * 2^23, rounded once, holds the code in its
+// lowest byte
 __device__ __forceinline__ uint32_t code4(const float* x, float inv) {
-    uint32_t w = 0;
+    uint32_t b[4];
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-        int c = (int)__builtin_rintf(x[j] * inv);
-        c = c > 127 ? 127 : (c < -127 ? -127 : c);
-        w |= ((uint32_t)c & 0xFFu) << (8 * j);
-    }
-    return w;
+    for (int j = 0; j < 4; j++) b[j] = __builtin_bit_cast(uint32_t, __builtin_fmaf(x[j], inv, 12582912.0f));
+    const uint32_t lo = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(b[3], b[2], 0x0c0c0400u);
+    return lo | (hi << 16);
 }
 
-// One wave takes 64 / GL rows (heads) of one token, GL lanes a row, 8 values a
-// lane: values e0 + [0, 4) and e1 + [0, 4) with, in split pairs (neox), e0 = 4 gl
-// and e1 = e0 + hd / 2, in interleaved pairs e0 = 8 gl and e1 = e0 + 4; either way
-// the lane's four pairs are its own and have the frequencies 4 gl + [0, 4).
-template <int GL, bool INT8>
-__global__ __launch_bounds__(256) void paged_front_kernel(PagedFrontArgs a) {
-    constexpr int RG = 64 / GL;                        // rows a wave takes at once
-    const int hd = a.head_dim, R = a.n_heads + 2 * a.n_kv;
-    const int groups = (R + RG - 1) / RG;
-    const int64_t gw = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int l = threadIdx.x & 63, sub = l / GL, gl = l % GL;
-    const int64_t t = gw / groups;
-    const int g = (int)(gw % groups);
-    if (t >= a.N) return;
-    const int slot = a.slots[t];
-    if (slot < 0 || slot >= a.n_slots) return;         // padding: nothing of this token is written
-    const int r = g * RG + sub;
-    const bool act = 8 * gl < hd && r < R;
-    const int kind = r < a.n_heads ? 0 : (r < a.n_heads + a.n_kv ? 1 : 2);   // q, k, v
-    const int head = kind == 0 ? r : (kind == 1 ? r - a.n_heads : r - a.n_heads - a.n_kv);
-    const int e0 = a.neox ? 4 * gl : 8 * gl, e1 = a.neox ? e0 + hd / 2 : e0 + 4;
-    const uint16_t* src = (kind == 0 ? a.q + t * a.q_stride : (kind == 1 ? a.k + t * a.k_stride : a.v + t * a.v_stride)) +
-                          (int64_t)head * hd;
-    u32x2f ra = {0u, 0u}, rb = {0u, 0u};
-    if (act) { ra = *(const u32x2f*)(src + e0); rb = *(const u32x2f*)(src + e1); }
-    float x[8];
+// sine and cosine of 2 pi turn 2^-32.  The nearest quarter turn goes into a swap and two
+// signs; what is left, |r| <= pi / 4, into the Taylor polynomials up to r^9 and r^8
+// (next terms: 2e-9 and 3e-8).  A third of the instructions of sincospif.
+__device__ __forceinline__ void sincos_turn(uint32_t turn, float& s, float& c) {
+    const uint32_t quarter = (turn + 0x20000000u) >> 30;
+    const float r = (float)(int32_t)(turn - (quarter << 30)) * 1.46291807926715968e-9f;     // 2 pi 2^-32
+    const float r2 = r * r;
+    const float ps = __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(__builtin_fmaf(r2, 1.0f / 362880.0f, -1.0f / 5040.0f), r2,
+                                    1.0f / 120.0f), r2, -1.0f / 6.0f), r2 * r, r);
+    const float pc = __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(__builtin_fmaf(r2, 1.0f / 40320.0f, -1.0f / 720.0f), r2,
+                                    1.0f / 24.0f), r2, -0.5f), r2, 1.0f);
+    const bool swap = quarter & 1u;
+    s = swap ? pc : ps;
+    c = swap ? ps : pc;
+    // quarters 2, 3 turn the sine's sign, 1, 2 the cosine's
+    s = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, s) ^ ((quarter & 2u) << 30));
+    c = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, c) ^ (((quarter + 1u) & 2u) << 30));
+}
+
+typedef float f32x4w __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint16_t u16x4w __attribute__((ext_vector_type(4), aligned(2)));
+
+// the lane's eight norm weights
+__device__ __forceinline__ void load_weights(const void* p, bool fp32, int e0, int e1, float (&w)[8]) {
+    if (fp32) {
+        const f32x4w x = *(const f32x4w*)((const float*)p + e0), y = *(const f32x4w*)((const float*)p + e1);
 #pragma unroll
-    for (int j = 0; j < 2; j++) {
-        x[2 * j] = f16_bits_to_f32(ra[j] & 0xFFFFu); x[2 * j + 1] = f16_bits_to_f32(ra[j] >> 16);
-        x[4 + 2 * j] = f16_bits_to_f32(rb[j] & 0xFFFFu); x[5 + 2 * j] = f16_bits_to_f32(rb[j] >> 16);
+        for (int j = 0; j < 4; j++) { w[j] = x[j]; w[4 + j] = y[j]; }
+    } else {
+        const u16x4w x = *(const u16x4w*)((const uint16_t*)p + e0), y = *(const u16x4w*)((const uint16_t*)p + e1);
+#pragma unroll
+        for (int j = 0; j < 4; j++) { w[j] = f16_bits_to_f32(x[j]); w[4 + j] = f16_bits_to_f32(y[j]); }
     }
-    if (a.q_norm) {
-        float ss = 0.0f;
+}
+
+// One wave takes 64 / GL rows (heads) of one token at a time, GL lanes a row, 8 values
+// a lane: values e0 + [0, 4) and e1 + [0, 4) with, in split pairs (neox), e0 = 4 gl
+// and e1 = e0 + hd / 2, in interleaved pairs e0 = 8 gl and e1 = e0 + 4; either way
+// the lane's four pairs are its own and have the frequencies 4 gl + [0, 4).  A wave
+// goes through iters groups of rows of its token, with the next group's values on
+// the way.  The kernel is bound by its instructions, not by the bytes, so what the
+// groups share is computed once: sines, cosines, and their products with the norm
+// weights, which a new kind of rows (q, then k) or a group of both renews.
+template <int GL, bool INT8, bool NEOX>
+__global__ __launch_bounds__(256) void paged_front_kernel(PagedFrontArgs a, int groups, int iters, int per) {
+    constexpr int RG = 64 / GL;                        // rows a wave takes at once
+    const int hd = a.head_dim, R = a.n_heads + 2 * a.n_kv, QK = a.n_heads + a.n_kv;
+    const unsigned tb = blockIdx.x / (unsigned)per;    // the block's four waves: four tokens, the same groups
+    const int64_t t = (int64_t)tb * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    if (t >= a.N) return;
+    const int g0 = (int)(blockIdx.x - tb * per) * iters, g1 = min(g0 + iters, groups);
+    const int l = threadIdx.x & 63, sub = l / GL, gl = l % GL;
+    const int e0 = NEOX ? 4 * gl : 8 * gl, e1 = NEOX ? e0 + hd / 2 : e0 + 4;
+    const bool in_row = 8 * gl < hd;
+    const float inv_hd = 1.0f / (float)hd;
+    const uint64_t qr = (uint64_t)(a.q + t * a.q_stride), kr0 = (uint64_t)(a.k + t * a.k_stride),
+                   vr0 = (uint64_t)(a.v + t * a.v_stride);
+
+    u32x2f ra = {0u, 0u}, rb = {0u, 0u};
+    auto load = [&](int g) {
+        const int r = g * RG + sub;
+        if (!in_row || r >= R) return;
+        const int kr = r - a.n_heads, vr = kr - a.n_kv;
+        typedef const __attribute__((address_space(1))) u32x2f* global_t;
+        uint64_t src = qr + 2 * (uint64_t)(r * hd);
+        if (kr >= 0) src = kr0 + 2 * (uint64_t)(kr * hd);
+        if (vr >= 0) src = vr0 + 2 * (uint64_t)(vr * hd);
+        ra = *(global_t)(src + 2 * e0);
+        rb = *(global_t)(src + 2 * e1);
+    };
+    const int slot = a.slots[t], pos = a.positions[t];
+    load(g0);
+    float wq[8], wk[8];
 #pragma unroll
-        for (int j = 0; j < 8; j++) ss += x[j] * x[j];
-        ss = group_sum_dpp<GL>(ss);
-        if (kind < 2 && act) {
-            const void* w = kind == 0 ? a.q_norm : a.k_norm;
-            const float rrms = 1.0f / sqrtf(ss / (float)hd + a.eps);
+    for (int j = 0; j < 8; j++) wq[j] = wk[j] = 1.0f;
+    if (a.q_norm && in_row) {
+        load_weights(a.q_norm, a.norm_fp32 != 0, e0, e1, wq);
+        load_weights(a.k_norm, a.norm_fp32 != 0, e0, e1, wk);
+    }
+    uint64_t fr[4];
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const int e = j < 4 ? e0 + j : e1 + j - 4;
-                x[j] *= rrms * (a.norm_fp32 ? ((const float*)w)[e] : f16_bits_to_f32(((const uint16_t*)w)[e]));
+    for (int j = 0; j < 4; j++) fr[j] = a.rt.f[4 * gl + j];
+    __builtin_amdgcn_sched_barrier(0);
+    if (slot < 0 || slot >= a.n_slots) return;         // padding: nothing of this token is written
+
+    float sn[4], cs[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        // bits 32 to 63 of fr * pos; a negative position counts 2^32 too much above
+        const uint32_t f0 = (uint32_t)fr[j], f1 = (uint32_t)(fr[j] >> 32);
+        sincos_turn(__umulhi(f0, (uint32_t)pos) + f1 * (uint32_t)pos - (pos < 0 ? f0 : 0u), sn[j], cs[j]);
+    }
+    // pair (p, q) -> (p c0 - q s0, p s1 + q c1)
+    float c0[4] = {}, s0[4] = {}, c1[4] = {}, s1[4] = {};
+    int have = -1;                                     // kind of the rows that these are for: 0 q, 1 k, 2 a mixture
+    for (int g = g0; g < g1; g++) {
+        const int r = g * RG + sub, kr = r - a.n_heads, vr = kr - a.n_kv;
+        const bool act = in_row && r < R;
+        const int first = g * RG, last = first + RG - 1;
+        if (first < QK) {
+            const int kind = last < a.n_heads ? 0 : (first >= a.n_heads ? 1 : 2);
+            if (kind != have) {
+                have = kind;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const int p = NEOX ? j : 2 * j, q = NEOX ? 4 + j : 2 * j + 1;
+                    const float wp = kr < 0 ? wq[p] : wk[p], wz = kr < 0 ? wq[q] : wk[q];
+                    c0[j] = cs[j] * wp; s0[j] = sn[j] * wz; s1[j] = sn[j] * wp; c1[j] = cs[j] * wz;
+                }
             }
         }
-    }
-    if (kind < 2 && act) {
-        const int64_t pos = a.positions[t];
+        float x[8];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            // signed fraction of a turn in units of 2^-32; sin and cos of pi * (2 frac)
-            const int32_t fr = (int32_t)((a.rt.f[4 * gl + j] * (uint64_t)pos) >> 32);
-            float s, c;
-            sincospif((float)fr * 0x1p-31f, &s, &c);
-            float& p = a.neox ? x[j] : x[2 * j];
-            float& q = a.neox ? x[4 + j] : x[2 * j + 1];
-            const float u = p * c - q * s, w = p * s + q * c;
-            p = u;
-            q = w;
+        for (int j = 0; j < 2; j++) {
+            x[2 * j] = f16_bits_to_f32(ra[j] & 0xFFFFu); x[2 * j + 1] = f16_bits_to_f32(ra[j] >> 16);
+            x[4 + 2 * j] = f16_bits_to_f32(rb[j] & 0xFFFFu); x[5 + 2 * j] = f16_bits_to_f32(rb[j] >> 16);
         }
-    }
-    if (kind == 0) {
-        if (act) {
-            uint16_t* o = a.q_out + t * a.q_out_stride + (int64_t)head * hd;
+        if (g + 1 < g1) load(g + 1);
+        if (first < QK) {
+            float rrms = 1.0f;
+            if (a.q_norm) {
+                float ss = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 8; j++) ss += x[j] * x[j];
+                rrms = __builtin_amdgcn_rsqf(group_sum_dpp<GL>(ss) * inv_hd + a.eps);     // 1 ulp
+            }
+            if (vr < 0) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    float &p = x[NEOX ? j : 2 * j], &q = x[NEOX ? 4 + j : 2 * j + 1];
+                    const float y = p * rrms, z = q * rrms;
+                    p = y * c0[j] - z * s0[j];
+                    q = y * s1[j] + z * c1[j];
+                }
+            }
+        }
+        if (kr < 0 && act) {
+            uint16_t* o = a.q_out + t * a.q_out_stride + r * hd;
             *(u32x2f*)(o + e0) = pack4(x);
             *(u32x2f*)(o + e1) = pack4(x + 4);
         }
-    }
-    const int64_t row = (int64_t)slot * a.n_kv + head;
-    void* pages = kind == 1 ? a.k_pages : a.v_pages;
-    if (INT8) {
-        uint32_t mb = 0;
+        if (last < a.n_heads) continue;                // only q heads in this group
+        const int64_t row = (int64_t)slot * a.n_kv + (vr < 0 ? kr : vr);
+        void* pages = vr < 0 ? a.k_pages : a.v_pages;
+        if (INT8) {
+            uint32_t mb = 0;
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const uint32_t b = __builtin_bit_cast(uint32_t, x[j]) & 0x7FFFFFFFu;
-            mb = b > mb ? b : mb;
+            for (int j = 0; j < 8; j++) mb = max(mb, __builtin_bit_cast(uint32_t, x[j]) & 0x7FFFFFFFu);
+            mb = group_max_dpp<GL>(mb);
+            if (kr >= 0 && act) {
+                const float mx = __builtin_bit_cast(float, mb);
+                const bool fine = mb < 0x7F800000u;    // a row with a NaN or an infinity reads as NaN
+                const bool some = fine && mx > 1e-35f; // below: 127 / mx overflows; the row is zero
+                const float rc = __builtin_amdgcn_rcpf(mx), i0 = 127.0f * rc;
+                const float inv = __builtin_fmaf(__builtin_fmaf(-i0, mx, 127.0f), rc, i0);   // 127 / mx to the nearest
+                int8_t* o = (int8_t*)pages + row * a.cache_head_dim;
+                *(uint32_t*)(o + e0) = some ? code4(x, inv) : 0u;
+                *(uint32_t*)(o + e1) = some ? code4(x + 4, inv) : 0u;
+                if (gl == 0) (vr < 0 ? a.k_scales : a.v_scales)[row] = fine ? mx / 127.0f : __builtin_nanf("");
+            }
+        } else if (kr >= 0 && act) {
+            uint16_t* o = (uint16_t*)pages + row * a.cache_head_dim;
+            *(u32x2f*)(o + e0) = pack4(x);
+            *(u32x2f*)(o + e1) = pack4(x + 4);
         }
-        mb = group_max_dpp<GL>(mb);
-        if (kind > 0 && act) {
-            const float mx = __builtin_bit_cast(float, mb);
-            const bool fine = mb < 0x7F800000u;        // a row with a NaN or an infinity reads as NaN
-            const float inv = fine && mx > 1e-35f ? 127.0f / mx : 0.0f;
-            int8_t* o = (int8_t*)pages + row * a.cache_head_dim;
-            *(uint32_t*)(o + e0) = fine ? code4(x, inv) : 0u;
-            *(uint32_t*)(o + e1) = fine ? code4(x + 4, inv) : 0u;
-            if (gl == 0) (kind == 1 ? a.k_scales : a.v_scales)[row] = fine ? mx / 127.0f : __builtin_nanf("");
-        }
-    } else if (kind > 0 && act) {
-        uint16_t* o = (uint16_t*)pages + row * a.cache_head_dim;
-        *(u32x2f*)(o + e0) = pack4(x);
-        *(u32x2f*)(o + e1) = pack4(x + 4);
     }
 }
 
 namespace {
 int lanes_of(int hd) { return hd <= 32 ? 4 : (hd <= 64 ? 8 : 16); }
+int groups_of(const PagedFrontArgs& a) {
+    const int rg = 64 / lanes_of(a.head_dim);
+    return (a.n_heads + 2 * a.n_kv + rg - 1) / rg;
+}
+// Groups of rows per wave: one while the waves do not fill the card, more (up to
+// all of a token's) beyond that.
+int iters_of(const PagedFrontArgs& a) {
+    const int groups = groups_of(a);
+    const int64_t it = (int64_t)a.N * groups / 4096;
+    return it < 1 ? 1 : (it > groups ? groups : (int)it);
+}
 }  // namespace
 
 int64_t paged_front_blocks(const PagedFrontArgs& a) {
-    const int rg = 64 / lanes_of(a.head_dim);
-    const int64_t groups = (a.n_heads + 2 * (int64_t)a.n_kv + rg - 1) / rg;
-    return ((int64_t)a.N * groups + 3) / 4;
+    const int groups = groups_of(a), iters = iters_of(a);
+    return ((int64_t)a.N + 3) / 4 * ((groups + iters - 1) / iters);
+}
+
+template <int GL, bool INT8>
+static void front_go(const PagedFrontArgs& a, hipStream_t st) {
+    const dim3 grid((unsigned)paged_front_blocks(a));
+    const int groups = groups_of(a), iters = iters_of(a), per = (groups + iters - 1) / iters;
+    if (a.neox) hipLaunchKernelGGL((paged_front_kernel<GL, INT8, true>), grid, dim3(256), 0, st, a, groups, iters, per);
+    else        hipLaunchKernelGGL((paged_front_kernel<GL, INT8, false>), grid, dim3(256), 0, st, a, groups, iters, per);
 }
 
 hipError_t paged_front_launch(const PagedFrontArgs& a, hipStream_t st) {
-    const dim3 grid((unsigned)paged_front_blocks(a));
-#define FRONT_CASE(GL)                                                                              \
-    if (a.kv_int8) hipLaunchKernelGGL((paged_front_kernel<GL, true>), grid, dim3(256), 0, st, a);   \
-    else           hipLaunchKernelGGL((paged_front_kernel<GL, false>), grid, dim3(256), 0, st, a);
-    switch (lanes_of(a.head_dim)) {
-    case 4:  FRONT_CASE(4) break;
-    case 8:  FRONT_CASE(8) break;
-    default: FRONT_CASE(16) break;
+    switch (lanes_of(a.head_dim) + (a.kv_int8 ? 1 : 0)) {
+    case 4:  front_go<4, false>(a, st); break;
+    case 5:  front_go<4, true>(a, st); break;
+    case 8:  front_go<8, false>(a, st); break;
+    case 9:  front_go<8, true>(a, st); break;
+    case 16: front_go<16, false>(a, st); break;
+    default: front_go<16, true>(a, st); break;
     }
-#undef FRONT_CASE
     return hipGetLastError();
 }
 
