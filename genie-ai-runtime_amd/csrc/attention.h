@@ -43,6 +43,7 @@ constexpr int ATTN_MAX_WAVES = 8;
 constexpr int ATTN_MAX_SPLITS = 256;
 constexpr int ATTN_MAX_COLUMNS = 32;   // (token, head) columns of a prefill MFMA tile
 int attn_splits(int seq_len, int n_kv);
+bool attn_splitk_enabled();            // JLLM_SPLITK, read once
 // waves per decode workgroup for n_splits key ranges
 int attn_decode_waves(int n_splits);
 size_t attn_partials_floats(int n_heads, int n_splits, int head_dim);

@@ -18,7 +18,8 @@ constexpr int MAX_BATCH = 65535;                 // grid dimension
 
 bool attn_shape_ok(int B, int n_heads, int n_kv, int hd, int max_seq, int window) {
     return B >= 0 && B <= MAX_BATCH && n_kv > 0 && n_heads > 0 && n_heads % n_kv == 0 && n_heads / n_kv <= 16 &&
-           n_heads <= 4096 && hd > 0 && hd % 32 == 0 && hd <= 128 && max_seq >= 0 && window >= 0;
+           n_heads <= 4096 && hd > 0 && hd % 32 == 0 && hd <= 128 && max_seq >= 0 && window >= 0 &&
+           paged_attn_blocks(B, n_kv, max_seq, window) < SERVING_MAX_BLOCKS;
 }
 }  // namespace
 
@@ -61,7 +62,7 @@ int jllm_hip_qk_norm_rope_store_kv_paged(uint16_t* q_out, int64_t q_out_stride, 
     a.k_scales = k_scales; a.v_scales = v_scales; a.n_slots = n_slots; a.positions = positions; a.slots = slots;
     a.n_heads = n_heads; a.n_kv = n_kv_heads; a.head_dim = head_dim; a.cache_head_dim = cache_head_dim; a.N = N;
     a.eps = eps; a.norm_fp32 = norm_fp32 != 0; a.neox = neox != 0; a.kv_int8 = kv_int8 != 0;
-    if (paged_front_blocks(a) >= FRONT_MAX_BLOCKS) return refuse(tag, "too many tokens for one launch");
+    if (paged_front_blocks(a) >= SERVING_MAX_BLOCKS) return refuse(tag, "too many tokens for one launch");
     rope_turns(a.rt, head_dim, theta_base);
     return launch_status(paged_front_launch(a, (hipStream_t)stream), tag);
 }
@@ -82,9 +83,9 @@ int jllm_hip_flash_attention_decode_paged(uint16_t* out, const uint16_t* q, int6
     static const char tag[] = "flash_attention_decode_paged";
     if (!attn_shape_ok(B, n_heads, n_kv_heads, head_dim, max_seq, window))
         return refuse(tag, "need n_heads % n_kv_heads == 0, <= 16 q heads per KV head, head_dim a multiple of 32 up "
-                           "to 128, B <= 65535, max_seq >= 0 and window >= 0");
-    if (cache_head_dim < head_dim || ((int64_t)cache_head_dim * (kv_int8 ? 1 : 2)) % 16 != 0)
-        return refuse(tag, "need cache_head_dim >= head_dim and cache rows of a multiple of 16 bytes");
+                           "to 128, B <= 65535, max_seq >= 0, window >= 0 and fewer than 2^24 workgroups");
+    if (cache_head_dim < head_dim || cache_head_dim > 4096 || ((int64_t)cache_head_dim * (kv_int8 ? 1 : 2)) % 16 != 0)
+        return refuse(tag, "need head_dim <= cache_head_dim <= 4096 and cache rows of a multiple of 16 bytes");
     if (page_size < 16 || page_size > 4096 || (page_size & (page_size - 1)) || n_pages < 0 ||
         (int64_t)n_pages * page_size > INT32_MAX)
         return refuse(tag, "need page_size a power of two from 16 to 4096 and n_pages * page_size < 2^31");
@@ -139,6 +140,7 @@ int jllm_hip_logits_process(float* out, int64_t out_stride, const float* logits,
                            n_bias, mask, next_token};
     for (const void* p : words)
         if (!aligned(p, 4)) return refuse(tag, "pointers must be 4-byte aligned");
+    if ((int64_t)B * (((int64_t)V + 1023) / 1024) >= SERVING_MAX_BLOCKS) return refuse(tag, "too many logits for one launch");
     const int64_t need = next_token ? logits_workspace(B, V) : 0;
     if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 8)))
         return refuse(tag, "workspace: null, not 8-byte aligned or smaller than jllm_hip_logits_process_workspace says");

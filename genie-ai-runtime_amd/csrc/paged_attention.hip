@@ -6,7 +6,9 @@
 // over the keys t of the row: [max(0, len - window), len).  Key t lies in slot
 // t % page_size of page table[row][t / page_size].
 //
-// One pass over K and V, all query heads of a KV head together.  A wave takes
+// One pass over K and V, all query heads of a KV head together.  The keys of all
+// rows are dealt out to as many workgroups as the card holds, in equal parts whatever
+// the rows' lengths are (the host knows only their maximum), and joined.  A wave takes
 // tiles of 32 keys, two blocks of 16 (a page holds whole blocks, so a block is one
 // base address).  With lane (li = l & 15, lg = l >> 4) of v_mfma_f32_16x16x32_f16:
 //   S^T = K q^T   rows = keys, columns = heads: the lane gets the scores of head li
@@ -25,21 +27,23 @@
 // times 2^14 so that they become subnormal only below 2^-28 of the largest.
 // With int8 the V scales go into the exponent, e^(s_t - m) vs_t = 2^(s'_t + log2
 // vs_t), with a maximum of their own: no scale can overflow or swamp the others.
+#include "attention.h"
 #include "attn_common.h"
 #include "serving.h"
 
 namespace jllm_hip {
 
 typedef float f32x4p __attribute__((ext_vector_type(4)));
+template <typename T> using global_ptr = const __attribute__((address_space(1))) T*;
 
 constexpr int PA_TILE = 32;            // keys a wave takes at once
 constexpr int PA_BLOCK = 16;           // keys behind one base address
-constexpr int PA_MAX_CHUNK = 1024;     // 64 blocks: one lane each
+constexpr int PA_PASS = 1024;          // keys whose pages a wave looks up at once: a block per lane
 constexpr int PA_WAVES = 4;
+constexpr int PA_MAX_ROWS = 1024;      // rows that a workgroup counts through
+constexpr int PA_MIN_UNITS = 2;        // units per workgroup at least
 constexpr float PA_LIFT = 14.0f;       // log2 of the factor on fp16 weights
 constexpr float PA_LOG2E = 1.44269504088896340736f;
-
-bool attn_splitk_enabled();
 
 // maximum / sum over the four 16-lane rows, in every lane
 __device__ __forceinline__ float rows_op(float v, bool sum) {
@@ -60,15 +64,59 @@ __device__ __forceinline__ u32x2a codes_to_h4(uint32_t w) {
     return u32x2a{__builtin_amdgcn_perm(u, u, 0x0c010c00u), __builtin_amdgcn_perm(u, u, 0x0c030c02u)};
 }
 
+// How the keys are dealt out.  A unit is a tile for each of the waves that share a
+// KV head.
+//   whole: a workgroup per row (and heads): writes the row's output itself
+//   else: the units of all rows, one row behind the other, cut into nw equal parts
+//     whatever the rows' lengths are; a part may hold pieces of several rows, a row
+//     pieces of several parts.  Piece (part w, row b) has partial w + b.  A row in
+//     one piece is written by its workgroup, the others by the join.
+struct PagedPlan { int whole, nw, heads; };
+
+struct RowKeys { int lo, base, len; };                 // keys [lo, len); base: lo rounded down to a block
+__device__ __forceinline__ RowKeys row_keys(const PagedAttnArgs& a, int len) {
+    RowKeys r;
+    r.len = len < 0 ? 0 : (len > a.max_seq ? a.max_seq : len);
+    r.lo = a.window > 0 && r.len > a.window ? r.len - a.window : 0;
+    r.base = r.lo & ~(PA_BLOCK - 1);
+    return r;
+}
+__device__ __forceinline__ int row_units(const RowKeys& r, int unit) { return (int)(((unsigned)(r.len - r.base) + unit - 1) / (unsigned)unit); }
+
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_add(int v) { return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false); }
+// inclusive prefix sum over the wave
+__device__ __forceinline__ int wave_scan(int v) {
+    v = dpp_add<0x111, 0xF>(v);     // row_shr 1, 2, 4, 8
+    v = dpp_add<0x112, 0xF>(v);
+    v = dpp_add<0x114, 0xF>(v);
+    v = dpp_add<0x118, 0xF>(v);
+    v = dpp_add<0x142, 0xA>(v);     // row_bcast 15 to rows 1 and 3
+    v = dpp_add<0x143, 0xC>(v);     // row_bcast 31 to rows 2 and 3
+    return v;
+}
+// units of rows r0 + [0, 64), one per lane
+__device__ __forceinline__ int group_units(const PagedAttnArgs& a, int r0, int l, int unit) {
+    return r0 + l < a.B ? row_units(row_keys(a, a.lens[r0 + l]), unit) : 0;
+}
+// first unit of part w when total units are cut into n parts
+__device__ __forceinline__ int part_begin(int total, int n, int w) {
+    const int q = total / n, rem = total - q * n;
+    return w * q + min(w, rem);
+}
+__device__ __forceinline__ int parts_of(int total, int nw) {
+    return max(1, min(nw, total / PA_MIN_UNITS));
+}
+
 // the weights' exponent base: a row without a finite score yet has base 0
 __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.0f : m; }
 
-struct PagedSplit { int chunk, splits; };
-
-template <bool INT8, int HD>
-__global__ __launch_bounds__(64 * PA_WAVES)
-void paged_attn_kernel(PagedAttnArgs a, int chunk, int S) {
+template <bool INT8, int HD, int HW>
+__global__ __launch_bounds__(64 * PA_WAVES, 3)
+void paged_attn_kernel(PagedAttnArgs a, PagedPlan plan) {
     constexpr int EB = INT8 ? 1 : 2;
+    constexpr int W = PA_WAVES / HW;                   // waves that share a KV head's keys
+    constexpr int UNIT = PA_TILE * W;
     constexpr int NST = HD / 32;                       // Q.K^T steps
     constexpr int KC = INT8 ? HD / 64 : HD / 32;       // 16-byte pieces of a K row per lane
     constexpr bool KT = INT8 && HD % 64 != 0;          // and an 8-byte one
@@ -76,44 +124,102 @@ void paged_attn_kernel(PagedAttnArgs a, int chunk, int S) {
     constexpr int V0 = HD == 96 ? 4 : NT;              // neighbouring d per lane, first part ...
     constexpr int V1 = NT - V0;                        // ... and second (from d = 64)
     constexpr int W0 = (V0 * EB + 3) / 4, W1 = (V1 * EB + 3) / 4, VW = W0 + W1;   // in words
+    constexpr int LD = HD + 4;
     extern __shared__ __attribute__((aligned(16))) float smem[];
 
-    const int kvh = blockIdx.x, split = blockIdx.y, b = blockIdx.z;
-    const int wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const unsigned hg = (unsigned)a.n_kv / HW, part = blockIdx.x / hg;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), hs = wave % HW, wv = wave / HW;
+    const int kvh = (int)(blockIdx.x - part * hg) * HW + hs;
     const int l = (int)threadIdx.x & 63, li = l & 15, lg = l >> 4;
     const int G = a.n_heads / a.n_kv;
-    int len = a.lens[b];
-    len = len < 0 ? 0 : (len > a.max_seq ? a.max_seq : len);
-    const int lo = a.window > 0 && len > a.window ? len - a.window : 0;
-    const int kv0 = (lo & ~(PA_BLOCK - 1)) + split * chunk, kv1 = min(kv0 + chunk, len);
+    float* sH = smem + (size_t)hs * W * (G * LD + 32);  // this KV head's part: numerators [W][G], m [W][16], l [W][16]
+    float* sO = sH + (size_t)wv * G * LD;
+    float* sML = sH + (size_t)W * G * LD;
+
+    // the part's units [at, end), and the rows that they lie in
+    int at = 0, end = 0, group = 0, mine = 0, incl = 0, before = 0;
+    if (!plan.whole) {
+        mine = group_units(a, 0, l, UNIT);
+        incl = wave_scan(mine);
+        int total = __builtin_amdgcn_readlane(incl, 63);
+        for (int r0 = 64; r0 < a.B; r0 += 64)
+            total += __builtin_amdgcn_readlane(wave_scan(group_units(a, r0, l, UNIT)), 63);
+        const int n = parts_of(total, plan.nw);
+        if ((int)part >= n) return;
+        at = part_begin(total, n, (int)part);
+        end = part_begin(total, n, (int)part + 1);
+    }
+
+  do {
+    int b = (int)part, u0 = 0, u1 = 0, units = 0;      // row, its units [u0, u1) that are this piece
+    if (!plan.whole) {
+        if (at >= end) return;
+        uint64_t beyond;
+        while (!(beyond = __builtin_amdgcn_ballot_w64(before + incl > at))) {
+            before += __builtin_amdgcn_readlane(incl, 63);
+            group += 64;
+            mine = group_units(a, group, l, UNIT);
+            incl = wave_scan(mine);
+        }
+        const int j = __builtin_ctzll(beyond);
+        b = group + j;
+        units = __builtin_amdgcn_readlane(mine, j);
+        const int first = before + __builtin_amdgcn_readlane(incl, j) - units;
+        u0 = at - first;
+        u1 = min(units, end - first);
+        at = first + u1;
+    }
+    const RowKeys rk_ = row_keys(a, a.lens[b]);
+    const int lo = rk_.lo;
+    if (plan.whole) u1 = units = row_units(rk_, UNIT);
     uint16_t* out = a.out + ((int64_t)b * a.n_heads + kvh * G) * HD;
-    if (kv0 >= kv1) {
-        // behind the row's end; an empty row is written here unless the join does it
-        if (S == 1)
-            for (int i = (int)threadIdx.x; i < G * HD; i += 64 * PA_WAVES) out[i] = 0;
+    if (units == 0) {                                  // (whole rows only: pieces have units)
+        for (int i = wv * 64 + l; i < G * HD; i += 64 * W) out[i] = 0;
         return;
     }
-    // lane j: slot of the first key of block j, and which blocks are there
-    const int nblk = (kv1 - kv0 + PA_BLOCK - 1) / PA_BLOCK;
-    const int bpos = kv0 + PA_BLOCK * min(l, nblk - 1);
-    const int page = a.table[b * a.table_stride + (bpos >> a.page_shift)];
-    const uint64_t there = __builtin_amdgcn_ballot_w64(l < nblk && (unsigned)page < (unsigned)a.n_pages);
-    const int slot0 = (page << a.page_shift) + (bpos & ((1 << a.page_shift) - 1));
+    // (key numbers up to 2^31: sums that may pass it are unsigned)
+    const int kv0 = rk_.base + u0 * UNIT, kv1 = (int)min((unsigned)rk_.base + (unsigned)(u1 * UNIT), (unsigned)rk_.len);
+
+    // Passes of 1024 keys: lane j looks up block j.  pg: the pages of the pass behind
+    // the current one.
+    auto look_up = [&](unsigned k0) {
+        const unsigned t = k0 + PA_BLOCK * l;
+        return t < (unsigned)kv1 ? a.table[b * a.table_stride + (t >> a.page_shift)] : -1;
+    };
+    int pass = kv0, slot0 = 0;
+    uint64_t there = 0, todo = 0;                      // blocks of the pass that are there; this wave's tiles of those (bit 2 i)
+    int pg = look_up(kv0);
+    auto enter = [&](unsigned k0) {
+        pass = (int)k0;
+        const unsigned t = k0 + PA_BLOCK * l;
+        there = __builtin_amdgcn_ballot_w64(t < (unsigned)kv1 && (unsigned)pg < (unsigned)a.n_pages);
+        slot0 = (pg << a.page_shift) + (int)(t & ((1u << a.page_shift) - 1));
+        todo = (there | (there >> 1)) & ((~(uint64_t)0 / (((uint64_t)1 << 2 * W) - 1)) << (2 * wv));
+        pg = look_up(k0 + PA_PASS);
+    };
+    enter(kv0);
 
     const uint32_t row = (uint32_t)a.n_kv * a.cache_head_dim * EB;      // bytes
     const int64_t hoff = (int64_t)kvh * a.cache_head_dim * EB;
 
-    // this wave's tiles wv, wv + W, ... of which a block is there: bit 2 i
-    uint64_t todo = (there | (there >> 1)) & ((~(uint64_t)0 / ((1 << 2 * PA_WAVES) - 1)) << (2 * wv));
+    // the wave's next tile: its first key, the slots of its blocks (a missing one
+    // takes the other's), which are there; p0 < 0: none
+    struct Tile { int p0, s0, s1; bool v0, v1; };
     auto next_tile = [&]() {
-        const int i = todo ? __builtin_ctzll(todo) / 2 : -1;
+        Tile x = {-1, 0, 0, false, false};
+        while (!todo) {
+            if ((unsigned)pass + PA_PASS >= (unsigned)kv1) return x;
+            enter((unsigned)pass + PA_PASS);
+        }
+        const int i = __builtin_ctzll(todo);
         todo &= todo - 1;
-        return i;
-    };
-    auto bases = [&](int i, int& s0, int& s1) {        // slots of a tile's blocks; a missing one takes the other's
-        const int x = __builtin_amdgcn_readlane(slot0, 2 * i), y = __builtin_amdgcn_readlane(slot0, 2 * i + 1);
-        s0 = (there >> (2 * i)) & 1 ? x : y;
-        s1 = (there >> (2 * i + 1)) & 1 ? y : x;
+        x.p0 = pass + PA_BLOCK * i;
+        x.v0 = (there >> i) & 1;
+        x.v1 = (there >> (i + 1)) & 1;
+        const int p = __builtin_amdgcn_readlane(slot0, i), q = __builtin_amdgcn_readlane(slot0, i + 1);
+        x.s0 = __builtin_amdgcn_readfirstlane(x.v0 ? p : q);     // (scalar base addresses)
+        x.s1 = __builtin_amdgcn_readfirstlane(x.v1 ? q : p);
+        return x;
     };
 
     // (zeroed: where a path leaves such registers undefined, this compiler has
@@ -122,14 +228,25 @@ void paged_attn_kernel(PagedAttnArgs a, int chunk, int S) {
     u32x2a rt[2] = {};
     uint32_t rv[8][VW] = {};
     float rs = 1.0f;
+    // A block's base address stays scalar, the lane's offset 32 bits (both opaque, or
+    // the compiler keeps a 64-bit address per load, which costs a wave per SIMD).
+    auto lane_offset = [](uint32_t x) {
+        asm("" : "+v"(x));
+        return x;
+    };
+    auto block_base = [&](const void* pages, int slot) {
+        uint64_t x = (uint64_t)pages + (uint64_t)((int64_t)slot * row + hoff);
+        asm("" : "+s"(x));
+        return x;
+    };
     auto load_k = [&](int s0, int s1) {
+        const uint32_t o = lane_offset((uint32_t)li * row + 16 * lg), o8 = lane_offset((uint32_t)li * row + 8 * lg);
 #pragma unroll
         for (int q = 0; q < 2; q++) {
-            const uint8_t* p = (const uint8_t*)a.k + (int64_t)(q ? s1 : s0) * row + hoff;
-            const uint32_t o = (uint32_t)li * row;
+            const uint64_t p = block_base(a.k, q ? s1 : s0);
 #pragma unroll
-            for (int c = 0; c < KC; c++) rk[q][c] = *(const u32x4a*)(p + (o + 64 * c + 16 * lg));
-            if (KT) rt[q] = *(const u32x2a*)(p + (o + 64 * KC + 8 * lg));
+            for (int c = 0; c < KC; c++) rk[q][c] = *(global_ptr<u32x4a>)(p + o + 64 * c);
+            if (KT) rt[q] = *(global_ptr<u32x2a>)(p + o8 + 64 * KC);
         }
         if (INT8) {
             // lane li: K (li < 8) or V scale of key 4 lg + li % 4 of block (li >> 2) & 1
@@ -139,28 +256,35 @@ void paged_attn_kernel(PagedAttnArgs a, int chunk, int S) {
         }
     };
     auto load_v = [&](int s0, int s1) {
+        uint32_t o[4], o1[4];
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const uint8_t* p = (const uint8_t*)a.v + (int64_t)(e < 4 ? s0 : s1) * row + hoff;
-            const uint32_t o = (uint32_t)(4 * lg + (e & 3)) * row;
-            const uint8_t* x = p + (o + V0 * EB * li);
-            if (V0 * EB == 16) { const u32x4a w = *(const u32x4a*)x; rv[e][0] = w.x; rv[e][1 % VW] = w.y; rv[e][2 % VW] = w.z; rv[e][3 % VW] = w.w; }
-            else if (V0 * EB == 8) { const u32x2a w = *(const u32x2a*)x; rv[e][0] = w.x; rv[e][1 % VW] = w.y; }
-            else if (V0 * EB == 4) rv[e][0] = *(const uint32_t*)x;
-            else rv[e][0] = *(const uint16_t*)x;
-            if (V1 > 0) {
-                const uint8_t* y = p + (o + 64 * EB + V1 * EB * li);
-                rv[e][VW - 1] = V1 * EB == 4 ? *(const uint32_t*)y : *(const uint16_t*)y;
+        for (int r = 0; r < 4; r++) {
+            o[r] = lane_offset((uint32_t)(4 * lg + r) * row + V0 * EB * li);
+            if (V1 > 0) o1[r] = lane_offset((uint32_t)(4 * lg + r) * row + V1 * EB * li);
+        }
+#pragma unroll
+        for (int q = 0; q < 2; q++) {
+            const uint64_t p = block_base(a.v, q ? s1 : s0);
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const uint64_t x = p + o[r];
+                uint32_t (&v)[VW] = rv[4 * q + r];
+                if (V0 * EB == 16) { const u32x4a w = *(global_ptr<u32x4a>)x; v[0] = w.x; v[1 % VW] = w.y; v[2 % VW] = w.z; v[3 % VW] = w.w; }
+                else if (V0 * EB == 8) { const u32x2a w = *(global_ptr<u32x2a>)x; v[0] = w.x; v[1 % VW] = w.y; }
+                else if (V0 * EB == 4) v[0] = *(global_ptr<uint32_t>)x;
+                else v[0] = *(global_ptr<uint16_t>)x;
+                if (V1 > 0) {
+                    const uint64_t y = p + o1[r] + 64 * EB;
+                    v[VW - 1] = V1 * EB == 4 ? *(global_ptr<uint32_t>)y : *(global_ptr<uint16_t>)y;
+                }
             }
         }
     };
 
-    int i = next_tile();
-    if (i >= 0) {
-        int s0, s1;
-        bases(i, s0, s1);
-        load_k(s0, s1);
-        load_v(s0, s1);
+    Tile cur = next_tile();
+    if (cur.p0 >= 0) {
+        load_k(cur.s0, cur.s1);
+        load_v(cur.s0, cur.s1);
     }
     __builtin_amdgcn_sched_barrier(0);
 
@@ -188,9 +312,9 @@ void paged_attn_kernel(PagedAttnArgs a, int chunk, int S) {
     for (int j = 0; j < NT; j++) acc[j] = f32x4p{};
     const h8 ones = __builtin_bit_cast(h8, u32x4a{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u});
 
-    while (i >= 0) {
-        const int p0 = kv0 + PA_TILE * i;
-        const bool v0 = (there >> (2 * i)) & 1, v1 = (there >> (2 * i + 1)) & 1;
+    while (cur.p0 >= 0) {
+        const int p0 = cur.p0;
+        const bool v0 = cur.v0, v1 = cur.v1;
         // 1. scores of the tile, in units of log2
         float s[8];
 #pragma unroll
@@ -215,12 +339,8 @@ void paged_attn_kernel(PagedAttnArgs a, int chunk, int S) {
         }
         // lanes li < 8: the K factor, li >= 8: log2 of the V scale
         const float sraw = rs;
-        const int in = next_tile();
-        int n0 = 0, n1 = 0;
-        if (in >= 0) {
-            bases(in, n0, n1);
-            load_k(n0, n1);
-        }
+        const Tile next = next_tile();
+        if (next.p0 >= 0) load_k(next.s0, next.s1);
         __builtin_amdgcn_sched_barrier(0);
         float sv = 0.0f;
         if (INT8) {
@@ -231,14 +351,14 @@ void paged_attn_kernel(PagedAttnArgs a, int chunk, int S) {
 #pragma unroll
             for (int e = 0; e < 8; e++) s[e] *= f0;
         }
-        const bool full = v0 && v1 && p0 >= lo && p0 + PA_TILE <= kv1;
+        const bool full = v0 && v1 && p0 >= lo && kv1 - p0 >= PA_TILE;
         uint32_t live = 0xFFu;                         // bit e: the lane's key e counts
         if (!full) {
             live = 0;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const int t = p0 + PA_BLOCK * (e >> 2) + 4 * lg + (e & 3);
-                if ((e < 4 ? v0 : v1) && t >= lo && t < kv1) live |= 1u << e;
+                const int o = PA_BLOCK * (e >> 2) + 4 * lg + (e & 3);      // key p0 + o
+                if ((e < 4 ? v0 : v1) && o >= lo - p0 && o < kv1 - p0) live |= 1u << e;
             }
 #pragma unroll
             for (int e = 0; e < 8; e++) s[e] = live >> e & 1 ? s[e] : -INFINITY;
@@ -316,8 +436,8 @@ void paged_attn_kernel(PagedAttnArgs a, int chunk, int S) {
         }
         if (INT8) wsum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pb, wsum, 0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
-        if (in >= 0) load_v(n0, n1);
-        i = in;
+        if (next.p0 >= 0) load_v(next.s0, next.s1);
+        cur = next;
     }
 
     // the wave's state: m, l, numerators; acc[j][r] is d = V0 (4 lg + r) + j, or 64 + V1 (4 lg + r) + j - V0
@@ -329,9 +449,6 @@ void paged_attn_kernel(PagedAttnArgs a, int chunk, int S) {
 #pragma unroll
             for (int r = 0; r < 4; r++) acc[j][r] = (acc[j][r] * 16777216.0f - 128.0f * wsum[0]) * f;
     }
-    constexpr int LD = HD + 4;
-    float* sO = smem + (size_t)wv * G * LD;
-    float* sML = smem + (size_t)PA_WAVES * G * LD;     // m [W][16], l [W][16]
     if (li < G) {
 #pragma unroll
         for (int j = 0; j < NT; j++)
@@ -339,137 +456,192 @@ void paged_attn_kernel(PagedAttnArgs a, int chunk, int S) {
             for (int r = 0; r < 4; r++)
                 sO[li * LD + (j < V0 ? V0 * (4 * lg + r) + j : 64 + V1 * (4 * lg + r) + j - V0)] = acc[j][r];
     }
-    if (l < 16) { sML[wv * 16 + l] = m; sML[(PA_WAVES + wv) * 16 + l] = L; }
+    if (l < 16) { sML[wv * 16 + l] = m; sML[(W + wv) * 16 + l] = L; }
     __syncthreads();
     // join of the waves in wave order
-    for (int e = (int)threadIdx.x; e < G * HD; e += 64 * PA_WAVES) {
+    for (int e = wv * 64 + l; e < G * HD; e += 64 * W) {
         const int h = e / HD, d = e % HD;
         float top = sML[h];
 #pragma unroll
-        for (int w = 1; w < PA_WAVES; w++) top = fmaxf(top, sML[w * 16 + h]);
+        for (int w = 1; w < W; w++) top = fmaxf(top, sML[w * 16 + h]);
         const float tb = base_of(top);
         float num = 0.0f, den = 0.0f;
 #pragma unroll
-        for (int w = 0; w < PA_WAVES; w++) {
+        for (int w = 0; w < W; w++) {
             const float f = __builtin_amdgcn_exp2f(sML[w * 16 + h] - tb);
-            num += f * smem[((size_t)w * G + h) * LD + d];
-            den += f * sML[(PA_WAVES + w) * 16 + h];
+            num += f * sH[((size_t)w * G + h) * LD + d];
+            den += f * sML[(W + w) * 16 + h];
         }
-        if (S == 1) {
+        if (u1 - u0 == units) {
             // no key of finite score: zero; a NaN stays
             out[e] = f32_to_f16_bits(den == 0.0f ? 0.0f : num / den);
         } else {
-            const int64_t at = ((int64_t)b * a.n_heads + kvh * G + h) * S + split;
-            const int64_t n = (int64_t)a.B * a.n_heads * S;
-            a.part[2 * n + at * HD + d] = num;
-            if (d == 0) { a.part[at] = top; a.part[n + at] = den; }
+            const int64_t n = (int64_t)(plan.nw + a.B) * a.n_heads, at_ = ((int64_t)part + b) * a.n_heads + kvh * G + h;
+            a.part[2 * n + at_ * HD + d] = num;
+            if (d == 0) { a.part[at_] = top; a.part[n + at_] = den; }
         }
     }
+    if (!plan.whole && at < end) __syncthreads();      // the next piece writes the states again
+  } while (!plan.whole);
 }
 
-// out = sum_s 2^(m_s - M) num_s / sum_s 2^(m_s - M) l_s over the splits that the
-// row has, in a fixed order: wave w of the head's workgroup adds splits w, w + NW,
-// ..., lane l d = 2 l and 2 l + 1; then the waves' sums in wave order.
+// out = sum_s 2^(m_s - M) num_s / sum_s 2^(m_s - M) l_s over the pieces of a row that
+// has several, in a fixed order: wave w of the head's workgroup adds pieces w, w + NW,
+// ..., lane l d = 2 l and 2 l + 1; then the waves' sums in wave order.  Rows without a
+// key are written here too.
 template <int NW>
-__global__ __launch_bounds__(64 * NW) void paged_join_kernel(PagedAttnArgs a, int chunk, int S) {
-    __shared__ float sM[NW];
-    __shared__ float sSum[NW][130];
-    const int b = blockIdx.y, h = blockIdx.x, hd = a.head_dim;
+__global__ __launch_bounds__(64 * NW) void paged_join_kernel(PagedAttnArgs a, PagedPlan plan) {
+    constexpr int AHEAD = 8;                           // pieces a wave has on the way
+    __shared__ float sTop[NW], sDen[NW];
+    __shared__ float sSum[NW][128];
+    const int b = blockIdx.y, h = blockIdx.x, hd = a.head_dim, unit = PA_TILE * (PA_WAVES / plan.heads);
     const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), l = (int)threadIdx.x & 63;
-    int len = a.lens[b];
-    len = len < 0 ? 0 : (len > a.max_seq ? a.max_seq : len);
-    const int lo = a.window > 0 && len > a.window ? len - a.window : 0;
-    const int ns = (len - (lo & ~(PA_BLOCK - 1)) + chunk - 1) / chunk;
-    const int64_t n = (int64_t)a.B * a.n_heads * S, at = ((int64_t)b * a.n_heads + h) * S;
+    int total = 0, first = 0, units = 0;
+    for (int r0 = 0; r0 < a.B; r0 += 64) {
+        const int mine = group_units(a, r0, l, unit), incl = wave_scan(mine);
+        if (b >= r0 && b < r0 + 64) {
+            units = __builtin_amdgcn_readlane(mine, b - r0);
+            first = total + __builtin_amdgcn_readlane(incl, b - r0) - units;
+        }
+        total += __builtin_amdgcn_readlane(incl, 63);
+    }
+    uint32_t* out = (uint32_t*)(a.out + ((int64_t)b * a.n_heads + h) * hd + 2 * l);
+    if (units == 0) {
+        if (w == 0 && 2 * l < hd) *out = 0;
+        return;
+    }
+    // part of a unit: the inverse of part_begin
+    const int n_ = parts_of(total, plan.nw), q = total / n_, rem = total - q * n_;
+    auto part_of = [&](int u) { return u < rem * (q + 1) ? u / (q + 1) : rem + (u - rem * (q + 1)) / q; };
+    const int w0 = part_of(first), ns = part_of(first + units - 1) - w0 + 1;
+    if (ns == 1) return;
+    const int64_t n = (int64_t)(plan.nw + a.B) * a.n_heads, at = ((int64_t)w0 + b) * a.n_heads + h;
+    const int64_t H = a.n_heads;
     const float* pm = a.part + at;
     const float* pl = a.part + n + at;
-    const float* pn = a.part + 2 * n + at * hd;
+    const float* pn = a.part + 2 * n + at * hd + (2 * l < hd ? 2 * l : 0);
+    // the first pieces' numerators set out together with the maxima
+    float2 v[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; i++) {
+        const int s = w + NW * i;
+        v[i] = s < ns ? *(const float2*)(pn + s * H * hd) : make_float2(0.0f, 0.0f);
+    }
     float top = -INFINITY;
-    for (int s = (int)threadIdx.x; s < ns; s += 64 * NW) top = fmaxf(top, pm[s]);
+    for (int s = (int)threadIdx.x; s < ns; s += 64 * NW) top = fmaxf(top, pm[s * H]);
     top = wave_max(top);
     if (NW > 1) {
-        if (l == 0) sM[w] = top;
+        if (l == 0) sTop[w] = top;
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < NW; i++) top = fmaxf(top, sM[i]);
+        for (int i = 0; i < NW; i++) top = fmaxf(top, sTop[i]);
     }
     const float tb = base_of(top);
     float den = 0.0f;
     float2 num = make_float2(0.0f, 0.0f);
-    const int d2 = 2 * l < hd ? 2 * l : 0;
-#pragma unroll 8
-    for (int s = w; s < ns; s += NW) {
-        const float f = __builtin_amdgcn_exp2f(pm[s] - tb);
-        const float2 v = *(const float2*)(pn + (int64_t)s * hd + d2);
-        den += f * pl[s];
-        num.x += f * v.x;
-        num.y += f * v.y;
+    for (int s0 = w; s0 < ns; s0 += NW * AHEAD) {
+        if (s0 > w)
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++)
+                v[i] = s0 + NW * i < ns ? *(const float2*)(pn + (s0 + NW * i) * H * hd) : make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) {
+            const int s = s0 + NW * i;
+            if (s >= ns) break;
+            const float f = __builtin_amdgcn_exp2f(pm[s * H] - tb);
+            den += f * pl[s * H];
+            num.x += f * v[i].x;
+            num.y += f * v[i].y;
+        }
     }
     if (NW > 1) {
         sSum[w][2 * l] = num.x;
         sSum[w][2 * l + 1] = num.y;
-        if (l == 0) sSum[w][128] = den;
+        if (l == 0) sDen[w] = den;
         __syncthreads();
         if (w > 0) return;
 #pragma unroll
         for (int i = 1; i < NW; i++) {
             num.x += sSum[i][2 * l];
             num.y += sSum[i][2 * l + 1];
-            den += sSum[i][128];
+            den += sDen[i];
         }
     }
     if (2 * l < hd) {
         const float x = den == 0.0f ? 0.0f : num.x / den, y = den == 0.0f ? 0.0f : num.y / den;
-        *(uint32_t*)(a.out + ((int64_t)b * a.n_heads + h) * hd + 2 * l) =
-            (uint32_t)f32_to_f16_bits(x) | ((uint32_t)f32_to_f16_bits(y) << 16);
+        *out = (uint32_t)f32_to_f16_bits(x) | ((uint32_t)f32_to_f16_bits(y) << 16);
     }
 }
 
 namespace {
-// Keys per workgroup: enough splits for 2048 workgroups when every row is as long
-// as it can be, at least a tile per wave, at most one block per lane.
-PagedSplit split_of(int B, int n_kv, int max_seq, int window) {
+// Whole rows where the longest is short: the join and its launch cost more than the
+// cut gains (INT8, 32 / 8 heads x 128: 1 row of 700 10.0 us against 11.2, 64 of 512
+// 17.6 against 25, 256 of 700 90 against 125; 8 fp16 rows of 1500 the other way,
+// 20.5 against 17.2).  Also where there are so many rows that counting through them
+// would cost more than their uneven lengths do.
+// Parts: as many as the card holds at once, three workgroups on each of 256 CUs.
+// Heads per workgroup: KV heads that run side by side read neighbouring pieces of
+// the same rows, which pays for int8's 128 bytes a head (48 rows of 2048: 51.9 us with
+// 2, 55.2 with 1; 131072 keys: 69 against 72), not for fp16's 256 (24 rows up to
+// 16384: 119.5 us with 1, 130 with 2), and only while the waves that are left per head
+// still have enough of a row (8192 keys, one row: 13.7 us with 1, 14.4 with 2).
+PagedPlan plan_of(int B, int n_kv, int max_seq, int window, bool int8) {
     int64_t span = max_seq;
     if (window > 0 && window + (int64_t)PA_BLOCK - 1 < span) span = window + (int64_t)PA_BLOCK - 1;
-    PagedSplit p;
-    if (span < 1) span = 1;
     const int64_t rows = (int64_t)(B > 0 ? B : 1) * n_kv;
-    const int64_t want = (2048 + rows - 1) / rows;
-    int64_t chunk = (span + want - 1) / want;
-    chunk = (chunk + PA_TILE * PA_WAVES - 1) / (PA_TILE * PA_WAVES) * (PA_TILE * PA_WAVES);
-    if (chunk > PA_MAX_CHUNK) chunk = PA_MAX_CHUNK;
-    p.chunk = (int)chunk;
-    p.splits = (int)((span + chunk - 1) / chunk);
+    PagedPlan p;
+    p.whole = !attn_splitk_enabled() || span <= PA_PASS || B > PA_MAX_ROWS ||
+              B * ((span + PA_TILE - 1) / PA_TILE) > (1 << 30);
+    if (p.whole) p.heads = rows >= 2048 ? 4 : (rows >= 512 ? 2 : 1);
+    else p.heads = int8 && B * span >= 65536 ? 2 : 1;
+    while (n_kv % p.heads) p.heads /= 2;
+    const int hg = n_kv / p.heads;
+    p.nw = p.whole ? 0 : (768 / hg > 1 ? 768 / hg : 1);
     return p;
+}
+
+template <bool INT8, int HD>
+void paged_go(const PagedAttnArgs& a, const PagedPlan& p, hipStream_t st) {
+    const dim3 grid((unsigned)(a.n_kv / p.heads) * (unsigned)(p.whole ? a.B : p.nw));
+    const size_t lds = (size_t)PA_WAVES * (a.n_heads / a.n_kv * (HD + 4) + 32) * 4;
+    switch (p.heads) {
+    case 1:  hipLaunchKernelGGL((paged_attn_kernel<INT8, HD, 1>), grid, dim3(64 * PA_WAVES), lds, st, a, p); break;
+    case 2:  hipLaunchKernelGGL((paged_attn_kernel<INT8, HD, 2>), grid, dim3(64 * PA_WAVES), lds, st, a, p); break;
+    default: hipLaunchKernelGGL((paged_attn_kernel<INT8, HD, 4>), grid, dim3(64 * PA_WAVES), lds, st, a, p); break;
+    }
 }
 }  // namespace
 
+int64_t paged_attn_blocks(int B, int n_kv, int max_seq, int window) {
+    // (of fp16, whose workgroups take fewer heads)
+    const PagedPlan p = plan_of(B, n_kv, max_seq, window, false);
+    return (int64_t)(n_kv / p.heads) * (p.whole ? B : p.nw);
+}
+
 int64_t paged_attn_workspace(int B, int n_heads, int n_kv, int head_dim, int max_seq, int window) {
-    const PagedSplit p = split_of(B, n_kv, max_seq, window);
-    if (p.splits == 1) return 0;
-    return ((int64_t)B * n_heads * p.splits * (2 + head_dim) * 4 + 15) & ~(int64_t)15;
+    // of int8, which has at least as many parts
+    const PagedPlan p = plan_of(B, n_kv, max_seq, window, true);
+    if (p.whole) return 0;
+    return ((int64_t)(p.nw + B) * n_heads * (2 + head_dim) * 4 + 15) & ~(int64_t)15;
 }
 
 hipError_t paged_attn_launch(const PagedAttnArgs& a, bool kv_int8, hipStream_t st) {
-    const PagedSplit p = split_of(a.B, a.n_kv, a.max_seq, a.window);
-    const int G = a.n_heads / a.n_kv;
-    const dim3 grid(a.n_kv, p.splits, a.B);
-    const size_t lds = ((size_t)PA_WAVES * G * (a.head_dim + 4) + PA_WAVES * 32) * 4;
-#define PAGED_CASE(HD)                                                                                                     \
-    if (kv_int8) hipLaunchKernelGGL((paged_attn_kernel<true, HD>), grid, dim3(64 * PA_WAVES), lds, st, a, p.chunk, p.splits);  \
-    else         hipLaunchKernelGGL((paged_attn_kernel<false, HD>), grid, dim3(64 * PA_WAVES), lds, st, a, p.chunk, p.splits);
-    switch (a.head_dim) {
-    case 32:  PAGED_CASE(32) break;
-    case 64:  PAGED_CASE(64) break;
-    case 96:  PAGED_CASE(96) break;
-    case 128: PAGED_CASE(128) break;
+    const PagedPlan p = plan_of(a.B, a.n_kv, a.max_seq, a.window, kv_int8);
+    switch (a.head_dim + (kv_int8 ? 1 : 0)) {
+    case 32:  paged_go<false, 32>(a, p, st); break;
+    case 33:  paged_go<true, 32>(a, p, st); break;
+    case 64:  paged_go<false, 64>(a, p, st); break;
+    case 65:  paged_go<true, 64>(a, p, st); break;
+    case 96:  paged_go<false, 96>(a, p, st); break;
+    case 97:  paged_go<true, 96>(a, p, st); break;
+    case 128: paged_go<false, 128>(a, p, st); break;
+    case 129: paged_go<true, 128>(a, p, st); break;
     default: return hipErrorInvalidValue;
     }
-#undef PAGED_CASE
     const hipError_t e = hipGetLastError();
-    if (e != hipSuccess || p.splits == 1) return e;
-    if (p.splits <= 16) hipLaunchKernelGGL((paged_join_kernel<1>), dim3(a.n_heads, a.B), dim3(64), 0, st, a, p.chunk, p.splits);
-    else                hipLaunchKernelGGL((paged_join_kernel<8>), dim3(a.n_heads, a.B), dim3(512), 0, st, a, p.chunk, p.splits);
+    if (e != hipSuccess || p.whole) return e;
+    if (p.nw <= 16 * a.B) hipLaunchKernelGGL((paged_join_kernel<1>), dim3(a.n_heads, a.B), dim3(64), 0, st, a, p);
+    else                  hipLaunchKernelGGL((paged_join_kernel<8>), dim3(a.n_heads, a.B), dim3(512), 0, st, a, p);
     return hipGetLastError();
 }
 

@@ -8,6 +8,8 @@
 
 namespace jllm_hip {
 
+constexpr int64_t SERVING_MAX_BLOCKS = (int64_t)1 << 24;   // 2^32 threads of 256-thread workgroups
+
 // ---- paged attention front ----
 
 // Rotary frequencies in turns: f[i] = theta^(-2i / head_dim) / 2 pi as a 64-bit
@@ -39,7 +41,6 @@ struct PagedFrontArgs {
     RopeTurns rt;
 };
 hipError_t paged_front_launch(const PagedFrontArgs& a, hipStream_t st);
-constexpr int64_t FRONT_MAX_BLOCKS = (int64_t)1 << 24;   // 2^32 threads of 256-thread workgroups
 int64_t paged_front_blocks(const PagedFrontArgs& a);
 
 // ---- paged decode attention ----
@@ -59,7 +60,9 @@ struct PagedAttnArgs {
     int n_pages, page_shift, B, n_heads, n_kv, head_dim, cache_head_dim, max_seq, window;
     float scale;
 };
-// bytes of partials for these sizes (0 when one split covers every row)
+// workgroups that a call of these sizes launches (below SERVING_MAX_BLOCKS)
+int64_t paged_attn_blocks(int B, int n_kv, int max_seq, int window);
+// bytes of partials for these sizes (0 when no row is cut)
 int64_t paged_attn_workspace(int B, int n_heads, int n_kv, int head_dim, int max_seq, int window);
 hipError_t paged_attn_launch(const PagedAttnArgs& a, bool kv_int8, hipStream_t st);
 

@@ -452,7 +452,8 @@ int jllm_hip_qk_norm_rope_store_kv_paged(uint16_t* q_out, int64_t q_out_stride, 
  * of one sequence (a prompt chunk) are passed as one row each, with the same
  * table row and growing lengths.
  * page_size a power of two from 16 to 4096; head_dim, heads and KV types
- * as in jllm_hip_flash_attention_decode, n_heads <= 4096 (scales NULL = 1.0).
+ * as in jllm_hip_flash_attention_decode, n_heads and cache_head_dim <= 4096
+ * (scales NULL = 1.0).
  * workspace: 16-byte aligned, any content, at least the bytes that
  * jllm_hip_flash_attention_decode_paged_workspace says, which returns a
  * negative JLLM_ERR_* for sizes that the operator refuses. */

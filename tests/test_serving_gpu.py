@@ -477,6 +477,33 @@ def test_attention_equal_scores_of_every_size(dev):
 
 
 @pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("H,KV,hd,lens,max_seq", [
+    (32, 32, 32, [40000], None),                       # parts of more than 1024 keys: several page look-ups
+    (4, 2, 32, [3000] + [5] * 70 + [0] * 60 + [1500] + [1] * 3, None),   # rows counted in groups of 64
+    (4, 2, 32, [0] * 130 + [2000], None),
+    (4, 2, 32, [0] * 70, 4000),                        # nothing to do
+    (4, 2, 32, [1, 0, 33, 2], 100000),                 # lengths far below what they could be
+    (2, 1, 32, [37, 90] * 500 + [3000, 0, 2000] + [1] * 97, None),       # more rows than are counted
+    (4, 1, 64, [1023, 1024, 1025, 2047, 2049, 1100], None)])
+def test_attention_parts(dev, int8, H, KV, hd, lens, max_seq):
+    print_case("paged attn parts", int8, H, KV, len(lens))
+    g = rng(H, KV, len(lens))
+    p = Pool(g, lens, KV, hd, 16, int8, max_seq=max_seq).upload()
+    q = (g.standard_normal((len(lens), H * hd)) * 1.2).astype(np.float16)
+    attn_check(p, host(attn_call(p, dev_(q), H, 0.15)), q, H, 0.15)
+
+
+@pytest.mark.parametrize("window", [1100, 3000])
+def test_attention_parts_with_a_window(dev, window):
+    H, KV, hd = 8, 2, 64
+    g = rng(window, 2)
+    lens = [9000, 1, 0, window, window + 1, window + 15, window + 16, 5000] + [2500] * 66
+    p = Pool(g, lens, KV, hd, 16, True).upload()
+    q = g.standard_normal((len(lens), H * hd)).astype(np.float16)
+    attn_check(p, host(attn_call(p, dev_(q), H, 0.125, window)), q, H, 0.125, window)
+
+
+@pytest.mark.parametrize("int8", [False, True])
 def test_attention_strided_q(dev, int8):
     H, KV, hd = 32, 8, 128
     g = rng(10)
