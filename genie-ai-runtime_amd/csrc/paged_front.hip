@@ -54,12 +54,14 @@ __device__ __forceinline__ uint32_t group_max_dpp(uint32_t v) {
 __device__ __forceinline__ u32x2f pack4(const float* x) {
     return u32x2f{h2_bits(half2_t{(_Float16)x[0], (_Float16)x[1]}), h2_bits(half2_t{(_Float16)x[2], (_Float16)x[3]})};
 }
-// the codes rint(x * inv): x * inv + 1.5 * 2^23, rounded once, holds the code in its
+// the codes rint(x * inv), the product rounded first as the KV quantiser does
+// (fp16_to_int8_kernel, convert.cu:26-69): adding 1.5 * 2^23 leaves the code in the
 // lowest byte
 __device__ __forceinline__ uint32_t code4(const float* x, float inv) {
+#pragma clang fp contract(off)
     uint32_t b[4];
 #pragma unroll
-    for (int j = 0; j < 4; j++) b[j] = __builtin_bit_cast(uint32_t, __builtin_fmaf(x[j], inv, 12582912.0f));
+    for (int j = 0; j < 4; j++) b[j] = __builtin_bit_cast(uint32_t, x[j] * inv + 12582912.0f);
     const uint32_t lo = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(b[3], b[2], 0x0c0c0400u);
     return lo | (hi << 16);
 }
@@ -217,8 +219,7 @@ __global__ __launch_bounds__(256) void paged_front_kernel(PagedFrontArgs a, int 
                 const float mx = __builtin_bit_cast(float, mb);
                 const bool fine = mb < 0x7F800000u;    // a row with a NaN or an infinity reads as NaN
                 const bool some = fine && mx > 1e-35f; // below: 127 / mx overflows; the row is zero
-                const float rc = __builtin_amdgcn_rcpf(mx), i0 = 127.0f * rc;
-                const float inv = __builtin_fmaf(__builtin_fmaf(-i0, mx, 127.0f), rc, i0);   // 127 / mx to the nearest
+                const float inv = 127.0f / mx;
                 int8_t* o = (int8_t*)pages + row * a.cache_head_dim;
                 *(uint32_t*)(o + e0) = some ? code4(x, inv) : 0u;
                 *(uint32_t*)(o + e1) = some ? code4(x + 4, inv) : 0u;

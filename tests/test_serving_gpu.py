@@ -206,6 +206,19 @@ def test_front_agrees_with_the_contiguous_front(dev):
         assert np.all(np.abs(a - b) <= 2.0 ** -10 * np.abs(b) + 8 * 200 * U + 2.0 ** -24)
 
 
+def test_front_values_get_the_codes_of_the_kv_quantiser(dev):
+    """V rows: the codes and scales of fp16_to_int8, bit for bit."""
+    H, KV, hd, N = 4, 8, 128, 300
+    g = rng(11)
+    x = (g.standard_normal((N, (H + 2 * KV) * hd)) * np.exp(g.standard_normal((N, 1)) * 3)).astype(np.float16)
+    (_, _, vp, _, vs), _, slots, _, _ = run_front(rng(11, 1), N, H, KV, hd, int8=True, x=x)
+    codes = torch.zeros((N * KV, hd), dtype=torch.int8, device="cuda:0")
+    scales = torch.zeros((N * KV,), device="cuda:0")
+    jllm.call("jllm_hip_fp16_to_int8", codes, scales, dev_(x[:, (H + KV) * hd:]), N * KV, hd)
+    assert np.array_equal(vp[slots].reshape(-1, hd), host(codes))
+    assert np.array_equal(vs[slots].reshape(-1), host(scales))
+
+
 # ---- attention ----------------------------------------------------------------------
 
 class Pool:
