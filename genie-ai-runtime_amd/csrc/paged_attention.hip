@@ -95,9 +95,10 @@ __device__ __forceinline__ int wave_scan(int v) {
     v = dpp_add<0x143, 0xC>(v);     // row_bcast 31 to rows 2 and 3
     return v;
 }
-// units of rows r0 + [0, 64), one per lane
-__device__ __forceinline__ int group_units(const PagedAttnArgs& a, int r0, int l, int unit) {
-    return r0 + l < a.B ? row_units(row_keys(a, a.lens[r0 + l]), unit) : 0;
+// length and units of rows r0 + [0, 64), one per lane
+__device__ __forceinline__ int group_units(const PagedAttnArgs& a, int r0, int l, int unit, int& len) {
+    len = r0 + l < a.B ? a.lens[r0 + l] : 0;
+    return row_units(row_keys(a, len), unit);
 }
 // first unit of part w when total units are cut into n parts
 __device__ __forceinline__ int part_begin(int total, int n, int w) {
@@ -137,13 +138,13 @@ void paged_attn_kernel(PagedAttnArgs a, PagedPlan plan) {
     float* sML = sH + (size_t)W * G * LD;
 
     // the part's units [at, end), and the rows that they lie in
-    int at = 0, end = 0, group = 0, mine = 0, incl = 0, before = 0;
+    int at = 0, end = 0, group = 0, lens = 0, mine = 0, incl = 0, before = 0;
     if (!plan.whole) {
-        mine = group_units(a, 0, l, UNIT);
+        mine = group_units(a, 0, l, UNIT, lens);
         incl = wave_scan(mine);
         int total = __builtin_amdgcn_readlane(incl, 63);
-        for (int r0 = 64; r0 < a.B; r0 += 64)
-            total += __builtin_amdgcn_readlane(wave_scan(group_units(a, r0, l, UNIT)), 63);
+        for (int r0 = 64, x; r0 < a.B; r0 += 64)
+            total += __builtin_amdgcn_readlane(wave_scan(group_units(a, r0, l, UNIT, x)), 63);
         const int n = parts_of(total, plan.nw);
         if ((int)part >= n) return;
         at = part_begin(total, n, (int)part);
@@ -151,37 +152,39 @@ void paged_attn_kernel(PagedAttnArgs a, PagedPlan plan) {
     }
 
   do {
-    int b = (int)part, u0 = 0, u1 = 0, units = 0;      // row, its units [u0, u1) that are this piece
-    if (!plan.whole) {
+    int b = (int)part, u0 = 0, u1 = 0, units = 0, len; // row, its units [u0, u1) that are this piece
+    if (plan.whole) {
+        len = a.lens[b];
+    } else {
         if (at >= end) return;
         uint64_t beyond;
         while (!(beyond = __builtin_amdgcn_ballot_w64(before + incl > at))) {
             before += __builtin_amdgcn_readlane(incl, 63);
             group += 64;
-            mine = group_units(a, group, l, UNIT);
+            mine = group_units(a, group, l, UNIT, lens);
             incl = wave_scan(mine);
         }
         const int j = __builtin_ctzll(beyond);
         b = group + j;
         units = __builtin_amdgcn_readlane(mine, j);
+        len = __builtin_amdgcn_readlane(lens, j);
         const int first = before + __builtin_amdgcn_readlane(incl, j) - units;
         u0 = at - first;
         u1 = min(units, end - first);
         at = first + u1;
     }
-    const RowKeys rk_ = row_keys(a, a.lens[b]);
-    const int lo = rk_.lo;
-    if (plan.whole) u1 = units = row_units(rk_, UNIT);
+    const RowKeys keys = row_keys(a, len);
+    const int lo = keys.lo;
+    if (plan.whole) u1 = units = row_units(keys, UNIT);
     uint16_t* out = a.out + ((int64_t)b * a.n_heads + kvh * G) * HD;
     if (units == 0) {                                  // (whole rows only: pieces have units)
         for (int i = wv * 64 + l; i < G * HD; i += 64 * W) out[i] = 0;
         return;
     }
     // (key numbers up to 2^31: sums that may pass it are unsigned)
-    const int kv0 = rk_.base + u0 * UNIT, kv1 = (int)min((unsigned)rk_.base + (unsigned)(u1 * UNIT), (unsigned)rk_.len);
+    const int kv0 = keys.base + u0 * UNIT, kv1 = (int)min((unsigned)keys.base + (unsigned)(u1 * UNIT), (unsigned)keys.len);
 
-    // Passes of 1024 keys: lane j looks up block j.  pg: the pages of the pass behind
-    // the current one.
+    // Passes of 1024 keys: lane j looks up block j, one pass ahead.
     auto look_up = [&](unsigned k0) {
         const unsigned t = k0 + PA_BLOCK * l;
         return t < (unsigned)kv1 ? a.table[b * a.table_stride + (t >> a.page_shift)] : -1;
@@ -498,7 +501,8 @@ __global__ __launch_bounds__(64 * NW) void paged_join_kernel(PagedAttnArgs a, Pa
     const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), l = (int)threadIdx.x & 63;
     int total = 0, first = 0, units = 0;
     for (int r0 = 0; r0 < a.B; r0 += 64) {
-        const int mine = group_units(a, r0, l, unit), incl = wave_scan(mine);
+        int len;
+        const int mine = group_units(a, r0, l, unit, len), incl = wave_scan(mine);
         if (b >= r0 && b < r0 + 64) {
             units = __builtin_amdgcn_readlane(mine, b - r0);
             first = total + __builtin_amdgcn_readlane(incl, b - r0) - units;
@@ -520,13 +524,20 @@ __global__ __launch_bounds__(64 * NW) void paged_join_kernel(PagedAttnArgs a, Pa
     const float* pm = a.part + at;
     const float* pl = a.part + n + at;
     const float* pn = a.part + 2 * n + at * hd + (2 * l < hd ? 2 * l : 0);
-    // the first pieces' numerators set out together with the maxima
+    // a wave's first pieces set out together with the maxima
     float2 v[AHEAD];
+    float pmax[AHEAD], psum[AHEAD];
+    auto load = [&](int s0) {
 #pragma unroll
-    for (int i = 0; i < AHEAD; i++) {
-        const int s = w + NW * i;
-        v[i] = s < ns ? *(const float2*)(pn + s * H * hd) : make_float2(0.0f, 0.0f);
-    }
+        for (int i = 0; i < AHEAD; i++) {
+            const int s = s0 + NW * i;
+            const bool is = s < ns;
+            v[i] = is ? *(const float2*)(pn + s * H * hd) : make_float2(0.0f, 0.0f);
+            pmax[i] = is ? pm[s * H] : -INFINITY;
+            psum[i] = is ? pl[s * H] : 0.0f;
+        }
+    };
+    load(w);
     float top = -INFINITY;
     for (int s = (int)threadIdx.x; s < ns; s += 64 * NW) top = fmaxf(top, pm[s * H]);
     top = wave_max(top);
@@ -540,16 +551,11 @@ __global__ __launch_bounds__(64 * NW) void paged_join_kernel(PagedAttnArgs a, Pa
     float den = 0.0f;
     float2 num = make_float2(0.0f, 0.0f);
     for (int s0 = w; s0 < ns; s0 += NW * AHEAD) {
-        if (s0 > w)
-#pragma unroll
-            for (int i = 0; i < AHEAD; i++)
-                v[i] = s0 + NW * i < ns ? *(const float2*)(pn + (s0 + NW * i) * H * hd) : make_float2(0.0f, 0.0f);
+        if (s0 > w) load(s0);
 #pragma unroll
         for (int i = 0; i < AHEAD; i++) {
-            const int s = s0 + NW * i;
-            if (s >= ns) break;
-            const float f = __builtin_amdgcn_exp2f(pm[s * H] - tb);
-            den += f * pl[s * H];
+            const float f = __builtin_amdgcn_exp2f(pmax[i] - tb);
+            den += f * psum[i];
             num.x += f * v[i].x;
             num.y += f * v[i].y;
         }
