@@ -182,7 +182,7 @@ void paged_attn_kernel(PagedAttnArgs a, PagedPlan plan) {
         return;
     }
     // (key numbers up to 2^31: sums that may pass it are unsigned)
-    const int kv0 = keys.base + u0 * UNIT, kv1 = (int)min((unsigned)keys.base + (unsigned)(u1 * UNIT), (unsigned)keys.len);
+    const int kv0 = keys.base + u0 * UNIT, kv1 = (int)min((unsigned)keys.base + (unsigned)u1 * UNIT, (unsigned)keys.len);
 
     // Passes of 1024 keys: lane j looks up block j, one pass ahead.
     auto look_up = [&](unsigned k0) {
@@ -581,10 +581,11 @@ __global__ __launch_bounds__(64 * NW) void paged_join_kernel(PagedAttnArgs a, Pa
 
 namespace {
 // Whole rows where the longest is short: the join and its launch cost more than the
-// cut gains (INT8, 32 / 8 heads x 128: 1 row of 700 10.0 us against 11.2, 64 of 512
-// 17.6 against 25, 256 of 700 90 against 125; 8 fp16 rows of 1500 the other way,
-// 20.5 against 17.2).  Also where there are so many rows that counting through them
-// would cost more than their uneven lengths do.
+// cut gains (32 / 8 heads x 128, whole against cut: 1 row of 400 fp16 keys 8.2 us
+// against 9.8, of 1000 13.2 against 9.9; 16 rows of 700 13.1 against 15.2; 64 of 1000
+// 54 against 60; 256 of 700 INT8 77 against 100; 8 of 1500 20.5 against 15.4).
+// Also where there are so many rows that counting through them would cost more than
+// their uneven lengths do.
 // Parts: as many as the card holds at once, three workgroups on each of 256 CUs.
 // Heads per workgroup: KV heads that run side by side read neighbouring pieces of
 // the same rows, which pays for int8's 128 bytes a head (48 rows of 2048: 51.9 us with
@@ -596,7 +597,7 @@ PagedPlan plan_of(int B, int n_kv, int max_seq, int window, bool int8) {
     if (window > 0 && window + (int64_t)PA_BLOCK - 1 < span) span = window + (int64_t)PA_BLOCK - 1;
     const int64_t rows = (int64_t)(B > 0 ? B : 1) * n_kv;
     PagedPlan p;
-    p.whole = !attn_splitk_enabled() || span <= PA_PASS || B > PA_MAX_ROWS ||
+    p.whole = !attn_splitk_enabled() || span <= (rows >= 128 ? 1024 : 768) || B > PA_MAX_ROWS ||
               B * ((span + PA_TILE - 1) / PA_TILE) > (1 << 30);
     if (p.whole) p.heads = rows >= 2048 ? 4 : (rows >= 512 ? 2 : 1);
     else p.heads = int8 && B * span >= 65536 ? 2 : 1;

@@ -428,7 +428,8 @@ int jllm_hip_gemm_dense_batched(uint16_t* out, const void* W, int wtype, const u
  * intermediate roundings and fp32 angle).  An int8 row that holds a NaN or an
  * infinity gets a NaN scale.
  * q_out, q, k, v: rows of q_out_stride, q_stride, ... halves (multiples of
- * 4: slices of a fused QKV buffer will do), 8-byte aligned; q_out may be q.
+ * 4: slices of a fused QKV buffer will do), 8-byte aligned; q_out may be q
+ * itself, otherwise its rows overlap none of the inputs'.
  * A token whose slot is outside [0, n_slots) is padding: its q_out row and
  * the pool are left as they are.  The slots of one call must be distinct.
  * head_dim a multiple of 8 up to 128; pages 16-byte aligned, cache rows a

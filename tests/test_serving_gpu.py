@@ -506,6 +506,67 @@ def test_attention_parts(dev, int8, H, KV, hd, lens, max_seq):
     attn_check(p, host(attn_call(p, dev_(q), H, 0.15)), q, H, 0.15)
 
 
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("hd", [32, 64, 96, 128])
+@pytest.mark.parametrize("H,KV,lens", [
+    (8, 8, [40, 17, 33, 0] * 64),                      # whole rows, four KV heads to a workgroup
+    (16, 8, [70, 1, 31] * 22),                         # two
+    (4, 2, [200, 90]),                                 # one
+    (4, 2, [3000, 2900, 40] * 8),                      # parts, int8: two
+    (2, 2, [1500, 700])])                              # parts, one
+def test_attention_heads_side_by_side(dev, int8, hd, H, KV, lens):
+    print_case("paged attn heads", int8, hd, H, KV, len(lens))
+    g = rng(hd, H, KV, len(lens))
+    p = Pool(g, lens, KV, hd, 16, int8).upload()
+    q = (g.standard_normal((len(lens), H * hd)) * 1.2).astype(np.float16)
+    scale = 1 / np.sqrt(hd)
+    attn_check(p, host(attn_call(p, dev_(q), H, scale)), q, H, scale)
+
+
+@pytest.mark.parametrize("page", [32, 256, 1024, 4096])
+def test_attention_page_sizes(dev, page):
+    g = rng(page)
+    p = Pool(g, [5000, 1, 0, 256, 1025], 2, 64, page, True).upload()
+    q = g.standard_normal((5, 8 * 64)).astype(np.float16)
+    attn_check(p, host(attn_call(p, dev_(q), 8, 0.125)), q, 8, 0.125)
+
+
+@pytest.mark.parametrize("lens", [[100, 250], [2500, 40, 300]])
+@pytest.mark.parametrize("which", ["ks", "vs"])
+def test_attention_scales_of_either_sign_and_one_null(dev, lens, which):
+    """Scales may be negative; with only one array given the other side's codes
+    stand for themselves."""
+    H, KV, hd = 8, 2, 64
+    g = rng(len(lens), ord(which[0]))
+    p = Pool(g, lens, KV, hd, 16, True)
+    sc = getattr(p, which)
+    sc *= np.where(g.random(sc.shape) < 0.4, -1.0, 1.0).astype(np.float32)
+    p.upload()
+    p.d[2 if which == "vs" else 3] = None
+    q = (g.standard_normal((len(lens), H * hd)) * 0.02).astype(np.float16)
+    for b, n in enumerate(lens):
+        pg, off = p.table[b][np.arange(n) // 16], np.arange(n) % 16
+        p.k[b] = p.kp[pg, off].astype(np.float64) * (p.ks[pg, off][..., None].astype(np.float64) if which == "ks" else 1)
+        p.v[b] = p.vp[pg, off].astype(np.float64) * (p.vs[pg, off][..., None].astype(np.float64) if which == "vs" else 1)
+    attn_check(p, host(attn_call(p, dev_(q), H, 0.125)), q, H, 0.125)
+
+
+@pytest.mark.parametrize("lens", [[50, 0, 3], [3000, 0, 20]])
+def test_attention_writes_its_rows_and_no_others(dev, lens):
+    H, KV, hd = 8, 2, 64
+    g = rng(77)
+    p = Pool(g, lens, KV, hd, 16, False).upload()
+    q = g.standard_normal((3, H * hd)).astype(np.float16)
+    out = torch.full((6, H * hd), 7.0, dtype=torch.float16, device="cuda:0")
+    need = jllm.lib().jllm_hip_flash_attention_decode_paged_workspace(3, H, KV, hd, p.max_seq, 0)
+    ws = torch.full((need + 64,), 0xFF, dtype=torch.uint8, device="cuda:0")
+    attn_call(p, dev_(q), H, 0.125, out=out[1:4], ws=ws[:max(need, 16)])
+    got = host(out)
+    attn_check(p, got[1:4], q, H, 0.125)
+    assert np.all(got[0] == 7.0) and np.all(got[4:] == 7.0)
+    assert np.all(host(ws)[need:] == 0xFF)             # the workspace is as large as it says
+
+
 @pytest.mark.parametrize("window", [1100, 3000])
 def test_attention_parts_with_a_window(dev, window):
     H, KV, hd = 8, 2, 64
