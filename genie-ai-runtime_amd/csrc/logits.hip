@@ -78,7 +78,7 @@ __global__ __launch_bounds__(LG_THREADS) void logits_kernel(LogitsArgs a) {
         if (i + 4 <= n) y[j] = *(const f32x4u*)(x + i);
         else
 #pragma unroll
-            for (int e = 0; e < 4; e++) y[j][e] = i + e < n ? x[i + e] : 0.0f;
+            for (int e = 0; e < 4; e++) y[j][e] = i + e < n ? x[i + e] : -INFINITY;
         word[j] = a.mask && i < n ? a.mask[b * a.mask_stride + ((c0 + i) >> 5)] : ~0u;
     }
     __builtin_amdgcn_sched_barrier(0);
@@ -91,24 +91,26 @@ __global__ __launch_bounds__(LG_THREADS) void logits_kernel(LogitsArgs a) {
     if (a.tokens) {
         const int nt = (int)max((int64_t)0, min((int64_t)a.n_tokens[b], a.token_stride));
         const int np = a.n_prompt ? max(0, min(a.n_prompt[b], nt)) : 0;
-        auto count = [&](int id, int i) {
-            const uint32_t at = (uint32_t)id - (uint32_t)c0;
+        auto count = [&](uint32_t at, int i) {             // at: place in this part
             if (at < (uint32_t)n && i < nt) {
                 if (i < np) atomicOr(&sCount[at], LG_PROMPT);
                 else atomicAdd(&sCount[at], 1u);
             }
         };
+        auto count4 = [&](i32x4u id, int i) {              // few of the ids fall into this part: one test for four
+            const uint32_t p0 = (uint32_t)id[0] - c0, p1 = (uint32_t)id[1] - c0, p2 = (uint32_t)id[2] - c0, p3 = (uint32_t)id[3] - c0;
+            if (min(min(p0, p1), min(p2, p3)) >= (uint32_t)n) return;
+            count(p0, i);
+            count(p1, i + 1);
+            count(p2, i + 2);
+            count(p3, i + 3);
+        };
         // whole fours of the row, then its last entries
         const int fours = (int)(a.token_stride & ~(int64_t)3);
-#pragma unroll
-        for (int e = 0; e < 4; e++) count(id4[e], 4 * t + e);
+        count4(id4, 4 * t);
 #pragma unroll 2
-        for (int i = 4 * (LG_THREADS + t); i < min(nt, fours); i += 4 * LG_THREADS) {
-            const i32x4u v = *(const i32x4u*)(ids + i);
-#pragma unroll
-            for (int e = 0; e < 4; e++) count(v[e], i + e);
-        }
-        if (fours + t < nt) count(ids[fours + t], fours + t);
+        for (int i = 4 * (LG_THREADS + t); i < min(nt, fours); i += 4 * LG_THREADS) count4(*(const i32x4u*)(ids + i), i);
+        if (fours + t < nt) count((uint32_t)ids[fours + t] - c0, fours + t);
     }
     if (a.bias_ids) {
         const int nb = (int)max((int64_t)0, min((int64_t)a.n_bias[b], a.bias_stride));
@@ -149,7 +151,9 @@ __global__ __launch_bounds__(LG_THREADS) void logits_kernel(LogitsArgs a) {
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             if (!(bits >> e & 1u)) y[j][e] = -INFINITY;
-            if (i + e < n && fabsf(y[j][e]) < INFINITY && (at < 0 || y[j][e] > best)) { best = y[j][e]; at = i + e; }
+            // (-inf, which masked tokens and those behind the row's end have, and NaN are
+            // not above the start value)
+            if (y[j][e] > best && y[j][e] < INFINITY) { best = y[j][e]; at = i + e; }
         }
         if (i + 4 <= n) *(f32x4u*)(out + i) = y[j];
         else
