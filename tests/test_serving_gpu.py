@@ -150,9 +150,10 @@ def test_front_nothing_but_padding(dev):
 
 
 @pytest.mark.parametrize("neox", [False, True])
-def test_front_far_positions(dev, neox):
+@pytest.mark.parametrize("theta", [1e4, 5e5, 1.5, 1.0, 0.75])
+def test_front_far_positions(dev, neox, theta):
     pos = [0, 1, 131071, 1 << 20, (1 << 24) + 1, 2 ** 31 - 1, -1, -2 ** 31]
-    r = run_front(rng(6), len(pos), 4, 2, 128, neox=neox, pos=pos, theta=1e4)
+    r = run_front(rng(6), len(pos), 4, 2, 128, neox=neox, pos=pos, theta=theta)
     check_front(*r, 4, 128, False)
 
 
