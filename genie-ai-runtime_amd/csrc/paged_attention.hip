@@ -31,7 +31,7 @@
 // Measured (32 / 8 heads x 128, both launches): 131072 fp16 keys of one row 103.7 us and
 // 24 rows of up to 16384 115.9 us (5.2 TB/s: the reads are the bound), 48 INT8 rows of
 // up to 4096 41.8 us (3.6 TB/s; start, join and the scales' lines are the rest), one
-// INT8 row of 700 10.1 us.
+// INT8 row of 700 9.1 us.
 #include "attention.h"
 #include "attn_common.h"
 #include "serving.h"
@@ -46,7 +46,6 @@ constexpr int PA_BLOCK = 16;           // keys behind one base address
 constexpr int PA_PASS = 1024;          // keys whose pages a wave looks up at once: a block per lane
 constexpr int PA_WAVES = 4;
 constexpr int PA_MAX_ROWS = 1024;      // rows that a workgroup counts through
-constexpr int PA_MIN_UNITS = 2;        // units per workgroup at least
 constexpr float PA_LIFT = 14.0f;       // log2 of the factor on fp16 weights
 constexpr float PA_LOG2E = 1.44269504088896340736f;
 
@@ -110,8 +109,12 @@ __device__ __forceinline__ int part_begin(int total, int n, int w) {
     const int q = total / n, rem = total - q * n;
     return w * q + min(w, rem);
 }
+// Parts of total units: a workgroup on every CU as long as each has a unit, more (up
+// to nw, three on every CU) only with two units each: 17 rows with a window of 1024
+// 9.6 us against 12.7 with two units from the start, one row of 2000 9.0 against 10.0,
+// but 8 rows of 1500 16.3 with single units throughout against 15.3.
 __device__ __forceinline__ int parts_of(int total, int nw) {
-    return max(1, min(nw, total / PA_MIN_UNITS));
+    return max(1, min(nw, max(total / 2, min(total, nw / 3))));
 }
 
 // the weights' exponent base: a row without a finite score yet has base 0
@@ -587,8 +590,9 @@ __global__ __launch_bounds__(64 * NW) void paged_join_kernel(PagedAttnArgs a, Pa
 namespace {
 // Whole rows where the longest is short: the join and its launch cost more than the
 // cut gains (32 / 8 heads x 128, whole against cut: 1 row of 400 fp16 keys 8.2 us
-// against 9.8, of 1000 13.2 against 9.9; 16 rows of 700 13.1 against 15.2; 64 of 1000
-// 54 against 60; 256 of 700 INT8 77 against 100; 8 of 1500 20.5 against 15.4).
+// against 9.8, of 600 9.7 against 8.8, of 1000 13.2 against 9.0; 16 rows of 700 13.1
+// against 15.2; 64 of 1000 54 against 60; 256 of 700 INT8 77 against 100; 8 of 1500 20.5
+// against 15.4).
 // Also where there are so many rows that counting through them would cost more than
 // their uneven lengths do.
 // Parts: as many as the card holds at once, three workgroups on each of 256 CUs.
@@ -602,7 +606,7 @@ PagedPlan plan_of(int B, int n_kv, int max_seq, int window, bool int8) {
     if (window > 0 && window + (int64_t)PA_BLOCK - 1 < span) span = window + (int64_t)PA_BLOCK - 1;
     const int64_t rows = (int64_t)(B > 0 ? B : 1) * n_kv;
     PagedPlan p;
-    p.whole = !attn_splitk_enabled() || span <= (rows >= 128 ? 1024 : 768) || B > PA_MAX_ROWS ||
+    p.whole = !attn_splitk_enabled() || span <= (rows >= 128 ? 1024 : 512) || B > PA_MAX_ROWS ||
               B * ((span + PA_TILE - 1) / PA_TILE) > (1 << 30);
     if (p.whole) p.heads = rows >= 2048 ? 4 : (rows >= 512 ? 2 : 1);
     else p.heads = int8 && B * span >= 65536 ? 2 : 1;
