@@ -446,12 +446,17 @@ int jllm_hip_qk_norm_rope_store_kv_paged(uint16_t* q_out, int64_t q_out_stride, 
  * attends to positions [0, seq_lens[b]) (the last `window` of them when
  * window > 0) of block_table row b, i.e. block_table + b * table_stride.
  * q rows of q_stride halves (a multiple of 8), out [B][n_heads * head_dim]
- * fp16.  A row of length <= 0 gives zeros; a length above max_seq counts as
+ * fp16, not overlapping q.  A row of length <= 0 gives zeros; a length above max_seq counts as
  * max_seq (host: the longest a row can be; it sizes the split of the keys).
  * The keys of a page id outside [0, n_pages) are skipped.  Slots of a page
  * behind the end of its sequence may hold anything.  Several query tokens
  * of one sequence (a prompt chunk) are passed as one row each, with the same
  * table row and growing lengths.
+ * The keys are dealt out to workgroups by the lengths of all rows, so a
+ * row's result can differ in its last bits with the rows beside it; the same
+ * call gives the same bits.  JLLM_SPLITK=0 in the environment (read once)
+ * leaves every row whole: slower where rows are few and long, and without
+ * a workspace.
  * page_size a power of two from 16 to 4096; head_dim, heads and KV types
  * as in jllm_hip_flash_attention_decode, n_heads and cache_head_dim <= 4096
  * (scales NULL = 1.0).

@@ -15,6 +15,10 @@ Tolerances, from the arithmetic (u = 2^-24, one fp32 rounding):
   then the output's own rounding 2^-11 |out| + 2^-25.
 * logits: the same fp32 operations in the same order, so the same bits.
 """
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 import torch
@@ -566,6 +570,24 @@ def test_attention_writes_its_rows_and_no_others(dev, lens):
     attn_check(p, got[1:4], q, H, 0.125)
     assert np.all(got[0] == 7.0) and np.all(got[4:] == 7.0)
     assert np.all(host(ws)[need:] == 0xFF)             # the workspace is as large as it says
+
+
+def test_attention_whole_rows_by_environment(dev):
+    """JLLM_SPLITK=0 (read once: a process of its own) leaves long rows whole."""
+    code = (
+        "import numpy as np, jllm, test_serving_gpu as t\n"
+        "assert jllm.lib().jllm_hip_flash_attention_decode_paged_workspace(3, 8, 4, 64, 9000, 0) == 0\n"
+        "for int8 in (False, True):\n"
+        "    g = t.rng(5)\n"
+        "    p = t.Pool(g, [9000, 0, 1500], 4, 64, 16, int8).upload()\n"
+        "    q = g.standard_normal((3, 8 * 64)).astype(np.float16)\n"
+        "    t.attn_check(p, t.host(t.attn_call(p, t.dev_(q), 8, 0.125)), q, 8, 0.125)\n"
+        "print('whole rows ok')\n")
+    here = os.path.dirname(os.path.abspath(__file__))
+    path = os.pathsep.join([here, os.path.join(os.path.dirname(here), "genie-ai-runtime_amd"), os.environ.get("PYTHONPATH", "")])
+    r = subprocess.run([sys.executable, "-c", code], env=dict(os.environ, JLLM_SPLITK="0", PYTHONPATH=path),
+                       capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and "whole rows ok" in r.stdout, r.stdout + r.stderr
 
 
 @pytest.mark.parametrize("window", [1100, 3000])
