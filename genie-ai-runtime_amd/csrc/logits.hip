@@ -158,7 +158,9 @@ __global__ __launch_bounds__(LG_THREADS) void logits_kernel(LogitsArgs a) {
             // not above the start value)
             if (y[j][e] > best && y[j][e] < INFINITY) { best = y[j][e]; at = i + e; }
         }
-        if (i + 4 <= n) *(f32x4u*)(out + i) = y[j];
+        // (not kept in the L2, where it would push out logits on their way in: 21.4 us
+        // -> 19.8 for 64 rows with lists and masks; loads marked so cost as much)
+        if (i + 4 <= n) __builtin_nontemporal_store(y[j], (f32x4u*)(out + i));
         else
 #pragma unroll
             for (int e = 0; e < 4; e++) if (i + e < n) out[i + e] = y[j][e];

@@ -40,6 +40,11 @@ namespace jllm_hip {
 
 typedef float f32x4p __attribute__((ext_vector_type(4)));
 template <typename T> using global_ptr = const __attribute__((address_space(1))) T*;
+template <bool ONCE, typename T>
+__device__ __forceinline__ T load_once(global_ptr<T> p) {
+    if (ONCE) return __builtin_nontemporal_load(p);
+    return *p;
+}
 
 constexpr int PA_TILE = 32;            // keys a wave takes at once
 constexpr int PA_BLOCK = 16;           // keys behind one base address
@@ -133,6 +138,12 @@ void paged_attn_kernel(PagedAttnArgs a, PagedPlan plan) {
     constexpr int V0 = HD == 96 ? 4 : NT;              // neighbouring d per lane, first part ...
     constexpr int V1 = NT - V0;                        // ... and second (from d = 64)
     constexpr int W0 = (V0 * EB + 3) / 4, W1 = (V1 * EB + 3) / 4, VW = W0 + W1;   // in words
+    // V rows that one load reads in whole lines are not kept in the caches, where they
+    // would push out lines of which half is still to be read (K's: a load reads 64
+    // bytes of a row): 24 fp16 rows of up to 16384 118 -> 110 us, 48 INT8 rows of up to
+    // 4096 44.2 -> 39.2.  Rows read in pieces, and K, lose by it (17 rows of head_dim
+    // 96: 9.9 -> 10.4; K 3 %).
+    constexpr bool VONCE = V1 == 0 && HD * EB % 128 == 0;
     constexpr int LD = HD + 4;
     extern __shared__ __attribute__((aligned(16))) float smem[];
 
@@ -280,8 +291,8 @@ void paged_attn_kernel(PagedAttnArgs a, PagedPlan plan) {
             for (int r = 0; r < 4; r++) {
                 const uint64_t x = p + o[r];
                 uint32_t (&v)[VW] = rv[4 * q + r];
-                if (V0 * EB == 16) { const u32x4a w = *(global_ptr<u32x4a>)x; v[0] = w.x; v[1 % VW] = w.y; v[2 % VW] = w.z; v[3 % VW] = w.w; }
-                else if (V0 * EB == 8) { const u32x2a w = *(global_ptr<u32x2a>)x; v[0] = w.x; v[1 % VW] = w.y; }
+                if (V0 * EB == 16) { const u32x4a w = load_once<VONCE>((global_ptr<u32x4a>)x); v[0] = w.x; v[1 % VW] = w.y; v[2 % VW] = w.z; v[3 % VW] = w.w; }
+                else if (V0 * EB == 8) { const u32x2a w = load_once<VONCE>((global_ptr<u32x2a>)x); v[0] = w.x; v[1 % VW] = w.y; }
                 else if (V0 * EB == 4) v[0] = *(global_ptr<uint32_t>)x;
                 else v[0] = *(global_ptr<uint16_t>)x;
                 if (V1 > 0) {
