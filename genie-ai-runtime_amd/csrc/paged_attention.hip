@@ -28,10 +28,10 @@
 // With int8 the V scales go into the exponent, e^(s_t - m) vs_t = 2^(s'_t + log2
 // vs_t), with a maximum of their own: no scale can overflow or swamp the others.
 //
-// Measured (32 / 8 heads x 128, both launches): 131072 fp16 keys of one row 103.7 us and
-// 24 rows of up to 16384 115.9 us (5.2 TB/s: the reads are the bound), 48 INT8 rows of
-// up to 4096 41.8 us (3.6 TB/s; start, join and the scales' lines are the rest), one
-// INT8 row of 700 9.1 us.
+// Measured (32 / 8 heads x 128, both launches): 131072 fp16 keys of one row 95.5 us and
+// 24 rows of up to 16384 106.8 us (5.6 TB/s: the reads are the bound), 48 INT8 rows of
+// up to 4096 38.9 us (3.8 TB/s; start, join and the scales' lines are the rest), one
+// INT8 row of 700 9.2 us.
 #include "attention.h"
 #include "attn_common.h"
 #include "serving.h"
