@@ -23,6 +23,12 @@ typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef int32_t i32x4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u32x4l __attribute__((ext_vector_type(4)));
 
+// entries of a list row that count (below 2^30: a count keeps its topmost bits, and
+// the loops' places stay ints)
+__device__ __forceinline__ int list_length(int n, int64_t stride) {
+    return (int)max((int64_t)0, min(min((int64_t)n, stride), (int64_t)1 << 30));
+}
+
 // (value, index) as one word that grows with the value and falls with the index;
 // 0: nothing to pick
 __device__ __forceinline__ uint64_t pick_key(float y, int i) {
@@ -66,13 +72,15 @@ __global__ __launch_bounds__(LG_THREADS) void logits_kernel(LogitsArgs a) {
     const float* x = a.x + b * a.x_stride + c0;
     float* out = a.out + b * a.out_stride + c0;
 
-    // the first round of the lists (rows are as long as their strides, so it may be
-    // read before it is known how much of it counts)
+    // The first round of the lists is read before it is known how much of it counts:
+    // up to the stride there is the row's or the next row's memory.  Behind the last
+    // row there may be none: it is read as far as it counts.
+    const bool ahead = b + 1 < a.B;
     const int32_t* ids = a.tokens + b * a.token_stride;
     const int32_t* bids = a.bias_ids + b * a.bias_stride;
     i32x4u id4 = {-1, -1, -1, -1};
-    if (a.tokens && 4 * t + 4 <= a.token_stride) id4 = *(const i32x4u*)(ids + 4 * t);
-    const int bid = a.bias_ids && t < a.bias_stride ? bids[t] : -1;
+    if (a.tokens && ahead && 4 * t + 4 <= a.token_stride) id4 = *(const i32x4u*)(ids + 4 * t);
+    int bid = a.bias_ids && ahead && t < a.bias_stride ? bids[t] : -1;
     f32x4u y[J];
     uint32_t word[J];
 #pragma unroll
@@ -92,7 +100,7 @@ __global__ __launch_bounds__(LG_THREADS) void logits_kernel(LogitsArgs a) {
         __syncthreads();
     }
     if (a.tokens) {
-        const int nt = (int)max((int64_t)0, min((int64_t)a.n_tokens[b], a.token_stride));
+        const int nt = list_length(a.n_tokens[b], a.token_stride);
         const int np = a.n_prompt ? max(0, min(a.n_prompt[b], nt)) : 0;
         auto count = [&](uint32_t at, int i) {             // at: place in this part
             if (at < (uint32_t)n && i < nt) {
@@ -108,19 +116,21 @@ __global__ __launch_bounds__(LG_THREADS) void logits_kernel(LogitsArgs a) {
             count(p2, i + 2);
             count(p3, i + 3);
         };
-        // whole fours of the row, then its last entries
-        const int fours = (int)(a.token_stride & ~(int64_t)3);
+        // whole fours of what may be read, then the last entries
+        const int fours = (ahead ? (int)a.token_stride : nt) & ~3;
+        if (!ahead && 4 * t < fours) id4 = *(const i32x4u*)(ids + 4 * t);
         count4(id4, 4 * t);
 #pragma unroll 2
         for (int i = 4 * (LG_THREADS + t); i < min(nt, fours); i += 4 * LG_THREADS) count4(*(const i32x4u*)(ids + i), i);
         if (fours + t < nt) count((uint32_t)ids[fours + t] - c0, fours + t);
     }
     if (a.bias_ids) {
-        const int nb = (int)max((int64_t)0, min((int64_t)a.n_bias[b], a.bias_stride));
+        const int nb = list_length(a.n_bias[b], a.bias_stride);
         auto list = [&](int id, int i) {
             const uint32_t at = (uint32_t)id - (uint32_t)c0;
             if (at < (uint32_t)n && i < nb) atomicMax(&sBias[at], (uint32_t)i + 1u);
         };
+        if (!ahead && t < nb) bid = bids[t];
         list(bid, t);
         for (int i = LG_THREADS + t; i < nb; i += LG_THREADS) list(bids[i], i);
     }

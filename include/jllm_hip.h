@@ -474,8 +474,8 @@ int jllm_hip_flash_attention_decode_paged(uint16_t* out, const uint16_t* q, int6
                                           void* stream);
 
 /* Penalties, biases and grammar masks on the fp32 logits [B][V] (rows of
- * logits_stride floats) of a batch, to out (rows of out_stride floats; may be
- * logits itself), and each row's greedy token.  Per row b, in this order:
+ * logits_stride floats) of a batch, to out (rows of out_stride floats;
+ * logits itself, or apart from it), and each row's greedy token.  Per row b, in this order:
  *   y = x > 0 ? x / repetition[b] : x * repetition[b]  for every token among
  *       the first n_tokens[b] of tokens + b * token_stride,
  *   y = y - frequency[b] * count, then y = y - presence[b], for those that
@@ -486,8 +486,9 @@ int jllm_hip_flash_attention_decode_paged(uint16_t* out, const uint16_t* q, int6
  *       mask + b * mask_stride is 0.
  * tokens, bias_ids, mask and next_token may be NULL (that part is skipped),
  * as may n_prompt (0), repetition (1), frequency and presence (0).  Counts
- * are held to [0, stride], n_prompt to [0, n_tokens]; ids outside [0, V) are
- * ignored.  next_token[b] = the lowest index of the largest finite y, -1 when
+ * are held to [0, min(stride, 2^30)], n_prompt to [0, n_tokens]; ids outside [0, V) are
+ * ignored.  Of all list rows but the last, entries up to the stride may be
+ * read.  next_token[b] = the lowest index of the largest finite y, -1 when
  * none is finite (a mask that leaves nothing); jllm_hip_dequant_embedding_rows
  * reads -1 as a zero row.
  * workspace (for next_token only): 8-byte aligned, at least the bytes that

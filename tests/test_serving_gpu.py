@@ -813,6 +813,28 @@ def test_logits_bad_ids_and_counts(dev):
     assert same(got, want) and np.array_equal(t, tok)
 
 
+@pytest.mark.parametrize("B,hist,bias", [(1, 1, 1), (1, 1500, 300), (3, 1027, 259), (2, 5, 7)])
+def test_logits_lists_inside_wider_rows(dev, B, hist, bias):
+    """Lists that are columns of wider arrays, the last row ending where the
+    array ends."""
+    g = rng(B, hist, bias)
+    V = 5000
+    x = g.standard_normal((B, V)).astype(np.float32)
+    c = logits_case(g, B, V, hist, bias, False)
+    c["n_tokens"][-1], c["n_bias"][-1] = hist, bias
+    want, tok = logits_ref(x, c)
+    wide, bwide = np.full((B, hist + 9), 17, np.int32), np.full((B, bias + 5), 17, np.int32)
+    bval = np.full((B, bias + 5), 1e6, np.float32)
+    wide[:, 9:], bwide[:, 5:], bval[:, 5:] = c["tokens"], c["bias_ids"], c["bias"]
+    d = {k: dev_(v) for k, v in c.items()}
+    W, BW, BV = dev_(wide)[:, 9:], dev_(bwide)[:, 5:], dev_(bval)[:, 5:]
+    out, t = torch.zeros((B, V), device="cuda:0"), torch.zeros((B,), dtype=torch.int32, device="cuda:0")
+    ws = torch.empty((max(jllm.lib().jllm_hip_logits_process_workspace(B, V), 16),), dtype=torch.uint8, device="cuda:0")
+    jllm.call("jllm_hip_logits_process", out, V, dev_(x), V, B, V, W, W.stride(0), d["n_prompt"], d["n_tokens"], d["rep"],
+              d["freq"], d["pres"], BW, BV, BW.stride(0), d["n_bias"], None, 0, t, ws, ws.numel())
+    assert same(host(out), want) and np.array_equal(host(t), tok)
+
+
 def test_logits_token_listed_often(dev):
     """One token 20000 times in the output, and a bias list of one token: the
     count is whole, the last bias counts."""
