@@ -50,7 +50,7 @@ constexpr int PA_TILE = 32;            // keys a wave takes at once
 constexpr int PA_BLOCK = 16;           // keys behind one base address
 constexpr int PA_PASS = 1024;          // keys whose pages a wave looks up at once: a block per lane
 constexpr int PA_WAVES = 4;
-constexpr int PA_MAX_ROWS = 1024;      // rows that a workgroup counts through
+constexpr int PA_MAX_ROWS = 1024;      // rows that a workgroup counts through (16 per lane)
 constexpr float PA_LIFT = 14.0f;       // log2 of the factor on fp16 weights
 constexpr float PA_LOG2E = 1.44269504088896340736f;
 
@@ -104,15 +104,20 @@ __device__ __forceinline__ int wave_scan(int v) {
     v = dpp_add<0x143, 0xC>(v);     // row_bcast 31 to rows 2 and 3
     return v;
 }
-// length and units of rows r0 + [0, 64), one per lane
-__device__ __forceinline__ int group_units(const PagedAttnArgs& a, int r0, int l, int unit, int& len) {
-    len = r0 + l < a.B ? a.lens[r0 + l] : 0;
+// units of row r, 0 behind the last row
+__device__ __forceinline__ int units_of(const PagedAttnArgs& a, int r, int unit, int& len) {
+    len = r < a.B ? a.lens[r] : 0;
     return row_units(row_keys(a, len), unit);
 }
 // first unit of part w when total units are cut into n parts
 __device__ __forceinline__ int part_begin(int total, int n, int w) {
     const int q = total / n, rem = total - q * n;
     return w * q + min(w, rem);
+}
+// the part that unit u falls into
+__device__ __forceinline__ int part_of(int total, int n, int u) {
+    const int q = total / n, rem = total - q * n;
+    return u < rem * (q + 1) ? u / (q + 1) : rem + (u - rem * (q + 1)) / q;
 }
 // Parts of total units: a workgroup on every CU as long as each has a unit, more (up
 // to nw, three on every CU) only with two units each: 17 rows with a window of 1024
@@ -125,7 +130,9 @@ __device__ __forceinline__ int parts_of(int total, int nw) {
 // the weights' exponent base: a row without a finite score yet has base 0
 __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.0f : m; }
 
-template <bool INT8, int HD, int HW>
+// WHOLE: a workgroup per row, without the code of the parts (one row of 30 keys 5.4 us
+// with both in one kernel)
+template <bool INT8, int HD, int HW, bool WHOLE>
 __global__ __launch_bounds__(64 * PA_WAVES, 3)
 void paged_attn_kernel(PagedAttnArgs a, PagedPlan plan) {
     constexpr int EB = INT8 ? 1 : 2;
@@ -150,51 +157,73 @@ void paged_attn_kernel(PagedAttnArgs a, PagedPlan plan) {
     const unsigned hg = (unsigned)a.n_kv / HW, part = blockIdx.x / hg;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), hs = wave % HW, wv = wave / HW;
     const int kvh = (int)(blockIdx.x - part * hg) * HW + hs;
-    const int l = (int)threadIdx.x & 63, li = l & 15, lg = l >> 4;
+    const int lane = (int)threadIdx.x & 63;
     const int G = a.n_heads / a.n_kv;
     float* sH = smem + (size_t)hs * W * (G * LD + 32);  // this KV head's part: numerators [W][G], m [W][16], l [W][16]
     float* sO = sH + (size_t)wv * G * LD;
     float* sML = sH + (size_t)W * G * LD;
 
     // the part's units [at, end), and the rows that they lie in
-    int at = 0, end = 0, group = 0, lens = 0, mine = 0, incl = 0, before = 0;
-    if (!plan.whole) {
-        mine = group_units(a, 0, l, UNIT, lens);
-        incl = wave_scan(mine);
-        int total = __builtin_amdgcn_readlane(incl, 63);
-        for (int r0 = 64, x; r0 < a.B; r0 += 64)
-            total += __builtin_amdgcn_readlane(wave_scan(group_units(a, r0, l, UNIT, x)), 63);
-        const int n = parts_of(total, plan.nw);
-        if ((int)part >= n) return;
-        at = part_begin(total, n, (int)part);
-        end = part_begin(total, n, (int)part + 1);
+    // (two levels: lane j counts rows j span + [0, span); of the group that a unit
+    // falls into the rows go to the lanes.  Up to 64 rows are one group.)
+    const int span = a.B <= 64 ? 64 : (a.B + 63) / 64;
+    int at = 0, end = 0, total = 0, n_parts = 1;
+    int group = 0, gincl = 0, lens = 0, incl = 0;       // incl: units up to the lane's row
+    auto enter_group = [&](int g, int base) {
+        group = g * span;
+        incl = base + wave_scan(lane < span ? units_of(a, group + lane, UNIT, lens) : 0);
+    };
+    if (!WHOLE) {
+        if (a.B <= 64) {
+            enter_group(0, 0);
+            total = __builtin_amdgcn_readlane(incl, 63);
+        } else {
+            int x, sum = 0;
+#pragma unroll 4
+            for (int i = 0; i < span; i++) sum += units_of(a, lane * span + i, UNIT, x);
+            gincl = wave_scan(sum);
+            total = __builtin_amdgcn_readlane(gincl, 63);
+        }
+        n_parts = parts_of(total, plan.nw);
+        if ((int)part >= n_parts) return;
+        at = part_begin(total, n_parts, (int)part);
+        end = part_begin(total, n_parts, (int)part + 1);
+        if (at >= end) return;
     }
 
   do {
+    // what follows from the lane is found anew for each piece: kept across the pieces it
+    // would take registers that the tiles need (24 fp16 rows of up to 16384 117 us, not 110)
+    int l = lane;
+    asm("" : "+v"(l));
+    const int li = l & 15, lg = l >> 4;
     int b = (int)part, u0 = 0, u1 = 0, units = 0, len; // row, its units [u0, u1) that are this piece
-    if (plan.whole) {
+    if (WHOLE) {
         len = a.lens[b];
     } else {
-        if (at >= end) return;
-        uint64_t beyond;
-        while (!(beyond = __builtin_amdgcn_ballot_w64(before + incl > at))) {
-            before += __builtin_amdgcn_readlane(incl, 63);
-            group += 64;
-            mine = group_units(a, group, l, UNIT, lens);
-            incl = wave_scan(mine);
+        uint64_t beyond = __builtin_amdgcn_ballot_w64(incl > at);
+        if (!beyond) {                                 // (more than 64 rows only)
+            const int g = __builtin_ctzll(__builtin_amdgcn_ballot_w64(gincl > at));
+            enter_group(g, g > 0 ? __builtin_amdgcn_readlane(gincl, g - 1) : 0);
+            beyond = __builtin_amdgcn_ballot_w64(incl > at);
         }
         const int j = __builtin_ctzll(beyond);
         b = group + j;
-        units = __builtin_amdgcn_readlane(mine, j);
         len = __builtin_amdgcn_readlane(lens, j);
-        const int first = before + __builtin_amdgcn_readlane(incl, j) - units;
+        units = row_units(row_keys(a, len), UNIT);
+        const int first = __builtin_amdgcn_readlane(incl, j) - units;
         u0 = at - first;
         u1 = min(units, end - first);
         at = first + u1;
+        // a row's first piece tells the join how many there are
+        if (u0 == 0 && blockIdx.x == part * hg && threadIdx.x == 0) {
+            int2* pieces = (int2*)(a.part + (int64_t)(plan.nw + a.B) * a.n_heads * (2 + HD));
+            pieces[b] = make_int2((int)part, u1 == units ? 1 : part_of(total, n_parts, first + units - 1) - (int)part + 1);
+        }
     }
     const RowKeys keys = row_keys(a, len);
     const int lo = keys.lo;
-    if (plan.whole) u1 = units = row_units(keys, UNIT);
+    if (WHOLE) u1 = units = row_units(keys, UNIT);
     uint16_t* out = a.out + ((int64_t)b * a.n_heads + kvh * G) * HD;
     if (units == 0) {                                  // (whole rows only: pieces have units)
         for (int i = wv * 64 + l; i < G * HD; i += 64 * W) out[i] = 0;
@@ -503,8 +532,8 @@ void paged_attn_kernel(PagedAttnArgs a, PagedPlan plan) {
             if (d == 0) { a.part[at_] = top; a.part[n + at_] = den; }
         }
     }
-    if (!plan.whole && at < end) __syncthreads();      // the next piece writes the states again
-  } while (!plan.whole);
+    if (!WHOLE && at < end) __syncthreads();      // the next piece writes the states again
+  } while (!WHOLE && at < end);
 }
 
 // out = sum_s 2^(m_s - M) num_s / sum_s 2^(m_s - M) l_s over the pieces of a row that
@@ -516,29 +545,18 @@ __global__ __launch_bounds__(64 * NW) void paged_join_kernel(PagedAttnArgs a, Pa
     constexpr int AHEAD = 8;                           // pieces a wave has on the way
     __shared__ float sTop[NW], sDen[NW];
     __shared__ float sSum[NW][128];
-    const int b = blockIdx.y, h = blockIdx.x, hd = a.head_dim, unit = PA_TILE * (PA_WAVES / plan.heads);
+    const int b = blockIdx.y, h = blockIdx.x, hd = a.head_dim;
     const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), l = (int)threadIdx.x & 63;
-    int total = 0, first = 0, units = 0;
-    for (int r0 = 0; r0 < a.B; r0 += 64) {
-        int len;
-        const int mine = group_units(a, r0, l, unit, len), incl = wave_scan(mine);
-        if (b >= r0 && b < r0 + 64) {
-            units = __builtin_amdgcn_readlane(mine, b - r0);
-            first = total + __builtin_amdgcn_readlane(incl, b - r0) - units;
-        }
-        total += __builtin_amdgcn_readlane(incl, 63);
-    }
+    const int64_t slots = (int64_t)(plan.nw + a.B) * a.n_heads;
+    const int2 pieces = *(const int2*)(a.part + slots * (2 + hd) + 2 * b);      // first part, count; of rows that have units
     uint32_t* out = (uint32_t*)(a.out + ((int64_t)b * a.n_heads + h) * hd + 2 * l);
-    if (units == 0) {
+    if (row_keys(a, a.lens[b]).len == 0) {
         if (w == 0 && 2 * l < hd) *out = 0;
         return;
     }
-    // part of a unit: the inverse of part_begin
-    const int n_ = parts_of(total, plan.nw), q = total / n_, rem = total - q * n_;
-    auto part_of = [&](int u) { return u < rem * (q + 1) ? u / (q + 1) : rem + (u - rem * (q + 1)) / q; };
-    const int w0 = part_of(first), ns = part_of(first + units - 1) - w0 + 1;
+    const int ns = pieces.y;
     if (ns == 1) return;
-    const int64_t n = (int64_t)(plan.nw + a.B) * a.n_heads, at = ((int64_t)w0 + b) * a.n_heads + h;
+    const int64_t n = slots, at = ((int64_t)pieces.x + b) * a.n_heads + h;
     const int64_t H = a.n_heads;
     const float* pm = a.part + at;
     const float* pl = a.part + n + at;
@@ -631,10 +649,12 @@ template <bool INT8, int HD>
 void paged_go(const PagedAttnArgs& a, const PagedPlan& p, hipStream_t st) {
     const dim3 grid((unsigned)(a.n_kv / p.heads) * (unsigned)(p.whole ? a.B : p.nw));
     const size_t lds = (size_t)PA_WAVES * (a.n_heads / a.n_kv * (HD + 4) + 32) * 4;
-    switch (p.heads) {
-    case 1:  hipLaunchKernelGGL((paged_attn_kernel<INT8, HD, 1>), grid, dim3(64 * PA_WAVES), lds, st, a, p); break;
-    case 2:  hipLaunchKernelGGL((paged_attn_kernel<INT8, HD, 2>), grid, dim3(64 * PA_WAVES), lds, st, a, p); break;
-    default: hipLaunchKernelGGL((paged_attn_kernel<INT8, HD, 4>), grid, dim3(64 * PA_WAVES), lds, st, a, p); break;
+    switch (p.heads + (p.whole ? 0 : 4)) {
+    case 1:  hipLaunchKernelGGL((paged_attn_kernel<INT8, HD, 1, true>), grid, dim3(64 * PA_WAVES), lds, st, a, p); break;
+    case 2:  hipLaunchKernelGGL((paged_attn_kernel<INT8, HD, 2, true>), grid, dim3(64 * PA_WAVES), lds, st, a, p); break;
+    case 4:  hipLaunchKernelGGL((paged_attn_kernel<INT8, HD, 4, true>), grid, dim3(64 * PA_WAVES), lds, st, a, p); break;
+    case 5:  hipLaunchKernelGGL((paged_attn_kernel<INT8, HD, 1, false>), grid, dim3(64 * PA_WAVES), lds, st, a, p); break;
+    default: hipLaunchKernelGGL((paged_attn_kernel<INT8, HD, 2, false>), grid, dim3(64 * PA_WAVES), lds, st, a, p); break;
     }
 }
 }  // namespace
@@ -649,7 +669,7 @@ int64_t paged_attn_workspace(int B, int n_heads, int n_kv, int head_dim, int max
     // of int8, which has at least as many parts
     const PagedPlan p = plan_of(B, n_kv, max_seq, window, true);
     if (p.whole) return 0;
-    return ((int64_t)(p.nw + B) * n_heads * (2 + head_dim) * 4 + 15) & ~(int64_t)15;
+    return ((int64_t)(p.nw + B) * n_heads * (2 + head_dim) * 4 + (int64_t)B * 8 + 15) & ~(int64_t)15;
 }
 
 hipError_t paged_attn_launch(const PagedAttnArgs& a, bool kv_int8, hipStream_t st) {
