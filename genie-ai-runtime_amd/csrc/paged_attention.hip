@@ -28,10 +28,10 @@
 // With int8 the V scales go into the exponent, e^(s_t - m) vs_t = 2^(s'_t + log2
 // vs_t), with a maximum of their own: no scale can overflow or swamp the others.
 //
-// Measured (32 / 8 heads x 128, both launches): 131072 fp16 keys of one row 95.5 us and
-// 24 rows of up to 16384 106.8 us (5.6 TB/s: the reads are the bound), 48 INT8 rows of
+// Measured (32 / 8 heads x 128, both launches): 131072 fp16 keys of one row 92 us and
+// 24 rows of up to 16384 102 us (5.8 TB/s: the reads are the bound), 48 INT8 rows of
 // up to 4096 38.9 us (3.8 TB/s; start, join and the scales' lines are the rest), one
-// INT8 row of 700 9.2 us.
+// INT8 row of 700 9.1 us.
 #include "attention.h"
 #include "attn_common.h"
 #include "serving.h"
@@ -79,7 +79,8 @@ __device__ __forceinline__ u32x2a codes_to_h4(uint32_t w) {
 //   else: the units of all rows, one row behind the other, cut into nw equal parts
 //     whatever the rows' lengths are; a part may hold pieces of several rows, a row
 //     pieces of several parts.  Piece (part w, row b) has partial w + b.  A row in
-//     one piece is written by its workgroup, the others by the join.
+//     one piece is written by its workgroup, the others by the join, which a row's
+//     first piece tells where they lie.
 struct PagedPlan { int whole, nw, heads; };
 
 struct RowKeys { int lo, base, len; };                 // keys [lo, len); base: lo rounded down to a block
@@ -622,15 +623,22 @@ namespace {
 // against 9.8, of 600 9.7 against 8.8, of 1000 13.2 against 9.0; 16 rows of 700 13.1
 // against 15.2; 64 of 1000 54 against 60; 256 of 700 INT8 77 against 100; 8 of 1500 20.5
 // against 15.4).
-// Also where there are so many rows that counting through them would cost more than
-// their uneven lengths do.
+// Also for more rows than PA_MAX_ROWS, which fill the card by themselves: 1500 rows up
+// to 2000 of 4 / 1 heads x 32 29 us whole, 38 cut; 1500 INT8 rows of 1100 of 16 / 2
+// heads 161 against 189, though 1100 fp16 rows up to 1200 101 against 84.
 // Parts: as many as the card holds at once, three workgroups on each of 256 CUs.
-// Heads per workgroup: KV heads that run side by side read neighbouring pieces of
-// the same rows, which pays for int8's 128 bytes a head (48 rows of 2048: 51.9 us with
-// 2, 55.2 with 1; 131072 keys: 69 against 72), not for fp16's 256 (24 rows up to
-// 16384: 119.5 us with 1, 130 with 2), and only while the waves that are left per head
-// still have enough of a row (8192 keys, one row: 13.7 us with 1, 14.4 with 2).
-PagedPlan plan_of(int B, int n_kv, int max_seq, int window, bool int8) {
+// Heads per workgroup: KV heads that run side by side read neighbouring pieces of the
+// same rows.  Pieces under 128 bytes share their lines (all lengths drawn; one head
+// against two: 128 INT8 rows up to 4000 of 8 heads x 64 78.5 us against 62.1, of 2 x 64
+// up to 8000 38.1 against 30.5; 128 fp16 rows up to 8000 of 4 x 32 60.3 against 45.4).
+// Whole lines gain little, and with few heads lose (24 fp16 rows of 8 x 128 up to 16384
+// 109.9 against 107.9, 16 INT8 rows of 8192 69 against 64; 64 INT8 rows up to 16000 of
+// 2 x 128 46.9 against 49.5, with 4 heads the same).  Both only while the two waves that
+// are left per head have enough of a row: the least number of keys over all heads from
+// which it pays is 2^19 up to 128 bytes and 2^20 from there (16 INT8 rows up to 2000 of
+// 2 x 64 9.3 against 9.8; 40 fp16 rows up to 1700 of 8 x 128 23.8 against 25.7).
+// piece: bytes of a key's row of one head.
+PagedPlan plan_of(int B, int n_kv, int max_seq, int window, int piece) {
     int64_t span = max_seq;
     if (window > 0 && window + (int64_t)PA_BLOCK - 1 < span) span = window + (int64_t)PA_BLOCK - 1;
     const int64_t rows = (int64_t)(B > 0 ? B : 1) * n_kv;
@@ -638,7 +646,7 @@ PagedPlan plan_of(int B, int n_kv, int max_seq, int window, bool int8) {
     p.whole = !attn_splitk_enabled() || span <= (rows >= 128 ? 1024 : 512) || B > PA_MAX_ROWS ||
               B * ((span + PA_TILE - 1) / PA_TILE) > (1 << 30);
     if (p.whole) p.heads = rows >= 2048 ? 4 : (rows >= 512 ? 2 : 1);
-    else p.heads = int8 && B * span >= 65536 ? 2 : 1;
+    else p.heads = rows * span >= (piece <= 128 ? 1 << 19 : 1 << 20) && (piece < 128 || n_kv >= 8) ? 2 : 1;
     while (n_kv % p.heads) p.heads /= 2;
     const int hg = n_kv / p.heads;
     p.nw = p.whole ? 0 : (768 / hg > 1 ? 768 / hg : 1);
@@ -660,20 +668,20 @@ void paged_go(const PagedAttnArgs& a, const PagedPlan& p, hipStream_t st) {
 }  // namespace
 
 int64_t paged_attn_blocks(int B, int n_kv, int max_seq, int window) {
-    // (of fp16, whose workgroups take fewer heads)
-    const PagedPlan p = plan_of(B, n_kv, max_seq, window, false);
+    // (of wide rows, whose workgroups take fewer heads)
+    const PagedPlan p = plan_of(B, n_kv, max_seq, window, 256);
     return (int64_t)(n_kv / p.heads) * (p.whole ? B : p.nw);
 }
 
 int64_t paged_attn_workspace(int B, int n_heads, int n_kv, int head_dim, int max_seq, int window) {
     // of int8, which has at least as many parts
-    const PagedPlan p = plan_of(B, n_kv, max_seq, window, true);
+    const PagedPlan p = plan_of(B, n_kv, max_seq, window, head_dim);
     if (p.whole) return 0;
     return ((int64_t)(p.nw + B) * n_heads * (2 + head_dim) * 4 + (int64_t)B * 8 + 15) & ~(int64_t)15;
 }
 
 hipError_t paged_attn_launch(const PagedAttnArgs& a, bool kv_int8, hipStream_t st) {
-    const PagedPlan p = plan_of(a.B, a.n_kv, a.max_seq, a.window, kv_int8);
+    const PagedPlan p = plan_of(a.B, a.n_kv, a.max_seq, a.window, a.head_dim * (kv_int8 ? 1 : 2));
     switch (a.head_dim + (kv_int8 ? 1 : 0)) {
     case 32:  paged_go<false, 32>(a, p, st); break;
     case 33:  paged_go<true, 32>(a, p, st); break;

@@ -528,6 +528,30 @@ def test_attention_heads_side_by_side(dev, int8, hd, H, KV, lens):
     attn_check(p, host(attn_call(p, dev_(q), H, scale)), q, H, scale)
 
 
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("H,KV,hd", [(16, 8, 128), (8, 8, 96), (24, 8, 64), (8, 8, 32), (16, 2, 32), (6, 6, 96)])
+def test_attention_parts_of_batches_that_could_be_long(dev, int8, H, KV, hd):
+    print_case("paged attn long bound", int8, H, KV, hd)
+    g = rng(H, KV, hd, 5)
+    lens = [3000, 0, 40, 1500, 700, 33, 1, 2900]
+    p = Pool(g, lens, KV, hd, 64, int8, max_seq=2 ** 17 // KV + 100).upload()
+    q = (g.standard_normal((len(lens), H * hd)) * 1.2).astype(np.float16)
+    scale = 1 / np.sqrt(hd)
+    attn_check(p, host(attn_call(p, dev_(q), H, scale)), q, H, scale)
+
+
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("B", [63, 64, 65, 127, 128, 129, 1000, 1023, 1024])
+def test_attention_parts_of_many_rows(dev, int8, B):
+    print_case("paged attn many rows", int8, B)
+    g = rng(B, 6)
+    lens = [int(n) for n in g.integers(0, 1200, B) * (g.random(B) < 0.4)]
+    lens[-1] = 1100
+    p = Pool(g, lens, 1, 32, 16, int8).upload()
+    q = (g.standard_normal((B, 2 * 32)) * 1.2).astype(np.float16)
+    attn_check(p, host(attn_call(p, dev_(q), 2, 0.2)), q, 2, 0.2)
+
+
 @pytest.mark.parametrize("page", [32, 256, 1024, 4096])
 def test_attention_page_sizes(dev, page):
     g = rng(page)
