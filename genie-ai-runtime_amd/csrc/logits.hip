@@ -9,7 +9,7 @@
 //   token = lowest index of the largest finite y, -1 when there is none
 //
 // Measured (both launches): 64 rows x 151936 with up to 4096 listed tokens, biases and
-// masks 19.2 us (4.1 TB/s), without any 15.3; 251 rows x 32003 16.1 us; one row 5.4 us.
+// masks 20.0 us (4.0 TB/s), without any 15.3; 251 rows x 32003 17.1 us; one row 5.6 us.
 #include "kq_common.h"
 #include "serving.h"
 
@@ -74,13 +74,15 @@ __global__ __launch_bounds__(LG_THREADS) void logits_kernel(LogitsArgs a) {
 
     // The first round of the lists is read before it is known how much of it counts:
     // up to the stride there is the row's or the next row's memory.  Behind the last
-    // row there may be none: it is read as far as it counts.
+    // row there may be none: it is read as far as it counts.  (By limits, not by a way
+    // of its own around the loads: 64 rows with lists and masks 20.3 us against 20.7.)
     const bool ahead = b + 1 < a.B;
+    const int first = ahead ? LG_THREADS : 0;
     const int32_t* ids = a.tokens + b * a.token_stride;
     const int32_t* bids = a.bias_ids + b * a.bias_stride;
     i32x4u id4 = {-1, -1, -1, -1};
-    if (a.tokens && ahead && 4 * t + 4 <= a.token_stride) id4 = *(const i32x4u*)(ids + 4 * t);
-    int bid = a.bias_ids && ahead && t < a.bias_stride ? bids[t] : -1;
+    if (a.tokens && 4 * t + 4 <= (ahead ? a.token_stride : 0)) id4 = *(const i32x4u*)(ids + 4 * t);
+    const int bid = a.bias_ids && t < (ahead ? a.bias_stride : 0) ? bids[t] : -1;
     f32x4u y[J];
     uint32_t word[J];
 #pragma unroll
@@ -118,10 +120,9 @@ __global__ __launch_bounds__(LG_THREADS) void logits_kernel(LogitsArgs a) {
         };
         // whole fours of what may be read, then the last entries
         const int fours = (ahead ? (int)a.token_stride : nt) & ~3;
-        if (!ahead && 4 * t < fours) id4 = *(const i32x4u*)(ids + 4 * t);
-        count4(id4, 4 * t);
+        count4(id4, 4 * t);                            // (the last row begins in the loop)
 #pragma unroll 2
-        for (int i = 4 * (LG_THREADS + t); i < min(nt, fours); i += 4 * LG_THREADS) count4(*(const i32x4u*)(ids + i), i);
+        for (int i = 4 * (first + t); i < min(nt, fours); i += 4 * LG_THREADS) count4(*(const i32x4u*)(ids + i), i);
         if (fours + t < nt) count((uint32_t)ids[fours + t] - c0, fours + t);
     }
     if (a.bias_ids) {
@@ -130,9 +131,8 @@ __global__ __launch_bounds__(LG_THREADS) void logits_kernel(LogitsArgs a) {
             const uint32_t at = (uint32_t)id - (uint32_t)c0;
             if (at < (uint32_t)n && i < nb) atomicMax(&sBias[at], (uint32_t)i + 1u);
         };
-        if (!ahead && t < nb) bid = bids[t];
         list(bid, t);
-        for (int i = LG_THREADS + t; i < nb; i += LG_THREADS) list(bids[i], i);
+        for (int i = first + t; i < nb; i += LG_THREADS) list(bids[i], i);
     }
     if (lists) __syncthreads();
     const float rep = a.tokens && a.repetition ? a.repetition[b] : 1.0f;
