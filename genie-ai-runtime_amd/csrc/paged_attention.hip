@@ -207,6 +207,7 @@ void paged_attn_kernel(PagedAttnArgs a, PagedPlan plan) {
             const int g = __builtin_ctzll(__builtin_amdgcn_ballot_w64(gincl > at));
             enter_group(g, g > 0 ? __builtin_amdgcn_readlane(gincl, g - 1) : 0);
             beyond = __builtin_amdgcn_ballot_w64(incl > at);
+            if (!beyond) return;                       // (lengths that changed since they were counted)
         }
         const int j = __builtin_ctzll(beyond);
         b = group + j;
@@ -549,15 +550,16 @@ __global__ __launch_bounds__(64 * NW) void paged_join_kernel(PagedAttnArgs a, Pa
     const int b = blockIdx.y, h = blockIdx.x, hd = a.head_dim;
     const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), l = (int)threadIdx.x & 63;
     const int64_t slots = (int64_t)(plan.nw + a.B) * a.n_heads;
-    const int2 pieces = *(const int2*)(a.part + slots * (2 + hd) + 2 * b);      // first part, count; of rows that have units
+    const int2 pieces = *(const int2*)(a.part + slots * (2 + hd) + 2 * b);      // first part, count; of rows that have keys
     uint32_t* out = (uint32_t*)(a.out + ((int64_t)b * a.n_heads + h) * hd + 2 * l);
     if (row_keys(a, a.lens[b]).len == 0) {
         if (w == 0 && 2 * l < hd) *out = 0;
         return;
     }
-    const int ns = pieces.y;
-    if (ns == 1) return;
-    const int64_t n = slots, at = ((int64_t)pieces.x + b) * a.n_heads + h;
+    // (bounded, so that lengths or a workspace that others write meanwhile spoil values only)
+    const int w0 = min(max(pieces.x, 0), plan.nw - 1), ns = min(pieces.y, plan.nw - w0);
+    if (ns <= 1) return;
+    const int64_t n = slots, at = ((int64_t)w0 + b) * a.n_heads + h;
     const int64_t H = a.n_heads;
     const float* pm = a.part + at;
     const float* pl = a.part + n + at;
