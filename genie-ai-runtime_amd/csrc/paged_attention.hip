@@ -26,7 +26,8 @@
 // the matrix cores (2^-12 of a weight, less than the output's own rounding),
 // times 2^14 so that they become subnormal only below 2^-28 of the largest.
 // With int8 the V scales go into the exponent, e^(s_t - m) vs_t = 2^(s'_t + log2
-// vs_t), with a maximum of their own: no scale can overflow or swamp the others.
+// vs_t), with a maximum of their own: no scale overflows the weights (below 1e34 the
+// fp32 sums neither) or swamps the others, and a scale of 0 is a weight of 0.
 //
 // Measured (32 / 8 heads x 128, both launches): 131072 fp16 keys of one row 92 us and
 // 24 rows of up to 16384 102 us (5.8 TB/s: the reads are the bound), 48 INT8 rows of
@@ -496,7 +497,9 @@ void paged_attn_kernel(PagedAttnArgs a, PagedPlan plan) {
     // the wave's state: m, l, numerators; acc[j][r] is d = V0 (4 lg + r) + j, or 64 + V1 (4 lg + r) + j - V0
     L = rows_op(L, true);
     if (INT8) {
-        const float f = __builtin_amdgcn_exp2f(base_of(M) - base_of(m) - PA_LIFT);
+        // (no V scale but 0: the numerators are 0, and with the base of an M of -inf the
+        // factor would be infinite under scores below -2^7)
+        const float f = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - base_of(m) - PA_LIFT);
 #pragma unroll
         for (int j = 0; j < NT; j++)
 #pragma unroll

@@ -1,0 +1,79 @@
+"""GPU checks of the batched serving operators where values are extreme: INT8
+scales that are zero, subnormal or NaN under scores far from zero.  References
+and tolerances are those of test_serving_gpu.
+"""
+import numpy as np
+import pytest
+import torch
+
+from gpu_util import print_case
+from test_serving_gpu import Pool, attn_call, attn_check, dev_, host, rng
+
+pytestmark = pytest.mark.gpu
+
+
+def far_pool(g, lens, KV, hd, sign, zero, tiny=0.0):
+    """INT8 sequences whose scores under q = 1, scale 1 / 8 all lie near 150 * sign;
+    the V scales where zero(b, t) holds are `tiny`."""
+    p = Pool(g, lens, KV, hd, 16, True)
+    for b, n in enumerate(lens):
+        pg, off = p.table[b][np.arange(n) // 16], np.arange(n) % 16
+        k = np.full((n, KV, hd), 100 * sign, np.int8)
+        k[:, :, 0] += g.integers(-9, 10, (n, KV)).astype(np.int8)
+        ks = np.full((n, KV), 150.0 * 8 / 100 / hd, np.float32)
+        p.kp[pg, off, :, :hd], p.ks[pg, off] = k, ks
+        gone = np.array([zero(b, t) for t in range(n)], bool)
+        p.vs[pg[gone], off[gone]] = tiny
+        p.k[b] = k * ks[..., None].astype(np.float64)
+        p.v[b] = p.vp[pg, off, :, :hd] * p.vs[pg, off][..., None].astype(np.float64)
+    return p.upload()
+
+
+ZERO = {
+    "all": lambda b, t: True,
+    "one tile": lambda b, t: 32 <= t < 64,             # of one wave, whole and cut
+    "one wave": lambda b, t: t // 32 % 4 == 1,
+    "one part": lambda b, t: 128 <= t < 256,
+    "but one key": lambda b, t: t != 40,
+    "half": lambda b, t: (t * 7919 >> 3) % 2 == 0,
+}
+
+
+@pytest.mark.parametrize("which", list(ZERO))
+@pytest.mark.parametrize("sign", [-1, 1])
+@pytest.mark.parametrize("lens", [[1, 64, 300, 41], [3000, 1, 0, 130, 700]])
+def test_attention_value_scales_of_zero(dev, which, sign, lens):
+    """Keys whose V scale is 0, as the front stores a zero V row, take part in the
+    softmax and add nothing, however far from zero the scores are.  (Scores: integer
+    sums, exact; four roundings after, 4 u * 150 * log2(e) < 2^-14 in a weight.)"""
+    print_case("zero V scales", which, sign, lens)
+    H, KV, hd = 8, 2, 64
+    p = far_pool(rng(len(lens), sign + 1), lens, KV, hd, sign, ZERO[which])
+    q = np.ones((len(lens), H * hd), np.float16)
+    attn_check(p, host(attn_call(p, dev_(q), H, 0.125)), q, H, 0.125)
+
+
+@pytest.mark.parametrize("lens", [[1, 64, 300], [3000, 5]])
+def test_attention_value_scales_below_the_normal_range(dev, lens):
+    """A scale of 1e-39 times a code is below every fp16: the key adds nothing."""
+    H, KV, hd = 8, 2, 64
+    p = far_pool(rng(len(lens), 5), lens, KV, hd, -1, ZERO["one wave"], tiny=1e-39)
+    q = np.ones((len(lens), H * hd), np.float16)
+    attn_check(p, host(attn_call(p, dev_(q), H, 0.125)), q, H, 0.125)
+
+
+@pytest.mark.parametrize("lens", [[1, 64, 300], [3000, 5]])
+@pytest.mark.parametrize("which", ["ks", "vs"])
+def test_attention_nan_scales_of_live_keys(dev, which, lens):
+    """A row stored from NaN or infinite values has a NaN scale: the heads of its KV
+    head are NaN, the others are as they were; beside zero V scales too."""
+    H, KV, hd = 8, 2, 64
+    p = far_pool(rng(len(lens), 6), lens, KV, hd, -1, ZERO["one wave"])
+    b, t = len(lens) - 1, lens[-1] - 1
+    getattr(p, which)[p.table[b, t // 16], t % 16, 1] = np.nan
+    p.upload()
+    q = np.ones((len(lens), H * hd), np.float16)
+    got = host(attn_call(p, dev_(q), H, 0.125)).reshape(len(lens), H, hd)
+    bad = np.zeros((len(lens), H), bool)
+    bad[b, H // 2:] = True
+    assert np.isnan(got[bad]).all() and np.isfinite(got[~bad]).all()
