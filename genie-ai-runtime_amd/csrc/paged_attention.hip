@@ -22,9 +22,13 @@
 //                 with a zero byte above it is the subnormal half (code + 128) 2^-24;
 //                 the 128 leaves through the accumulator's start value for K, and through
 //                 the sum of the weights for V).
-// Sums, maxima and accumulators are fp32.  The weights are rounded to fp16 for
-// the matrix cores (2^-12 of a weight, less than the output's own rounding),
-// times 2^14 so that they become subnormal only below 2^-28 of the largest.
+// Sums, maxima and accumulators are fp32.  For the matrix cores a weight is split into
+// two fp16 parts, each rounded down, as in the other attention kernels: together 2^-21
+// of the weight, so the output's rounding is the only one to 11 bits (with one part,
+// 2^-12 of sum w |v|, values that cancel lost their difference).  The second product
+// and the split cost 0.3 % of 24 fp16 rows of up to 16384, 1.5 % of 48 INT8 rows of up
+// to 4096 and at most 2.5 % (64 INT8 rows of 4 / 1 heads x 32, 15.2 us).  The parts are
+// of the weight times 2^14, so that they become subnormal only below 2^-28 of the largest.
 // With int8 the V scales go into the exponent, e^(s_t - m) vs_t = 2^(s'_t + log2
 // vs_t), with a maximum of their own: no scale overflows the weights (below 1e34 the
 // fp32 sums neither) or swamps the others, and a scale of 0 is a weight of 0.
@@ -52,7 +56,7 @@ constexpr int PA_BLOCK = 16;           // keys behind one base address
 constexpr int PA_PASS = 1024;          // keys whose pages a wave looks up at once: a block per lane
 constexpr int PA_WAVES = 4;
 constexpr int PA_MAX_ROWS = 1024;      // rows that a workgroup counts through (16 per lane)
-constexpr float PA_LIFT = 14.0f;       // log2 of the factor on fp16 weights
+constexpr float PA_LIFT = 16384.0f;    // factor on the weights' fp16 parts
 constexpr float PA_LOG2E = 1.44269504088896340736f;
 
 // maximum / sum over the four 16-lane rows, in every lane
@@ -427,7 +431,7 @@ void paged_attn_kernel(PagedAttnArgs a, PagedPlan plan) {
         float p[8], ps = 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            p[e] = __builtin_amdgcn_exp2f(s[e] - (INT8 ? mb : mb - PA_LIFT));
+            p[e] = __builtin_amdgcn_exp2f(s[e] - mb);
             ps += p[e];
         }
         L = L * corr + ps;
@@ -447,7 +451,7 @@ void paged_attn_kernel(PagedAttnArgs a, PagedPlan plan) {
             corr = __builtin_amdgcn_exp2f(M - Mb);
             M = Mn;
 #pragma unroll
-            for (int e = 0; e < 8; e++) p[e] = __builtin_amdgcn_exp2f(t[e] - (Mb - PA_LIFT));
+            for (int e = 0; e < 8; e++) p[e] = __builtin_amdgcn_exp2f(t[e] - Mb);
             // a negative V scale: its sign back onto the weight (no quantiser here writes one)
             if (__builtin_amdgcn_ballot_w64(li >= 8 && sraw < 0.0f)) {
                 p[0] = __builtin_copysignf(p[0], row_bcast<8>(sraw)); p[1] = __builtin_copysignf(p[1], row_bcast<9>(sraw));
@@ -462,9 +466,15 @@ void paged_attn_kernel(PagedAttnArgs a, PagedPlan plan) {
             for (int j = 0; j < NT; j++) acc[j] *= corr;
             if (INT8) wsum *= corr;
         }
-        h8 pb;
+        h8 pb, pl;                                     // p * PA_LIFT in two parts, each rounded down
 #pragma unroll
-        for (int e = 0; e < 8; e++) pb[e] = (_Float16)p[e];
+        for (int e = 0; e < 8; e += 2) {
+            const float x = p[e] * PA_LIFT, y = p[e + 1] * PA_LIFT;
+            const auto hi = __builtin_amdgcn_cvt_pkrtz(x, y);
+            const auto lo = __builtin_amdgcn_cvt_pkrtz(x - (float)hi[0], y - (float)hi[1]);
+            pb[e] = (_Float16)hi[0]; pb[e + 1] = (_Float16)hi[1];
+            pl[e] = (_Float16)lo[0]; pl[e + 1] = (_Float16)lo[1];
+        }
         // 3. O^T += V^T P^T
         if (!INT8 && !full) {                          // what a slot without a key holds may be NaN
 #pragma unroll
@@ -487,8 +497,12 @@ void paged_attn_kernel(PagedAttnArgs a, PagedPlan plan) {
 #pragma unroll
             for (int e = 0; e < 4; e++) va[e] = __builtin_amdgcn_perm(rv[2 * e + 1][w], rv[2 * e][w], sel);
             acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, va), pb, acc[j], 0, 0, 0);
+            acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, va), pl, acc[j], 0, 0, 0);
         }
-        if (INT8) wsum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pb, wsum, 0, 0, 0);
+        if (INT8) {
+            wsum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pb, wsum, 0, 0, 0);
+            wsum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pl, wsum, 0, 0, 0);
+        }
         __builtin_amdgcn_sched_barrier(0);
         if (next.p0 >= 0) load_v(next.s0, next.s1);
         cur = next;
@@ -499,11 +513,14 @@ void paged_attn_kernel(PagedAttnArgs a, PagedPlan plan) {
     if (INT8) {
         // (no V scale but 0: the numerators are 0, and with the base of an M of -inf the
         // factor would be infinite under scores below -2^7)
-        const float f = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - base_of(m) - PA_LIFT);
+        const float f = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - base_of(m)) * (1.0f / PA_LIFT);
 #pragma unroll
         for (int j = 0; j < NT; j++)
 #pragma unroll
             for (int r = 0; r < 4; r++) acc[j][r] = (acc[j][r] * 16777216.0f - 128.0f * wsum[0]) * f;
+    } else {
+#pragma unroll
+        for (int j = 0; j < NT; j++) acc[j] *= 1.0f / PA_LIFT;
     }
     if (li < G) {
 #pragma unroll

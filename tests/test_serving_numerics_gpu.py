@@ -1,13 +1,13 @@
 """GPU checks of the batched serving operators where values are extreme: INT8
-scales that are zero, subnormal or NaN under scores far from zero.  References
-and tolerances are those of test_serving_gpu.
+scales that are zero, subnormal or NaN under scores far from zero, values that
+cancel.  References and tolerances are those of test_serving_gpu where none is given.
 """
 import numpy as np
 import pytest
 import torch
 
 from gpu_util import print_case
-from test_serving_gpu import Pool, attn_call, attn_check, dev_, host, rng
+from test_serving_gpu import Pool, attn_call, attn_check, attn_ref, dev_, host, rng
 
 pytestmark = pytest.mark.gpu
 
@@ -77,3 +77,55 @@ def test_attention_nan_scales_of_live_keys(dev, which, lens):
     bad = np.zeros((len(lens), H), bool)
     bad[b, H // 2:] = True
     assert np.isnan(got[bad]).all() and np.isfinite(got[~bad]).all()
+
+
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("H,KV,hd", [(8, 2, 64), (32, 8, 128), (12, 1, 96), (4, 4, 32)])
+@pytest.mark.parametrize("lens", [[2, 3, 40, 300], [2, 700, 3000, 9]])
+def test_attention_weights_keep_more_than_fp16(dev, int8, H, KV, hd, lens):
+    """Values that nearly cancel: up to eight keys of a row have almost the same
+    weight and values of either sign, the others values of 0 and weights below 2^-28,
+    so the output is a small difference that weights of 11 bits do not have.
+
+    Error of a weight: 2^-21 where it is held in two fp16 parts, 2^-22 for exp2,
+    2^-21 for the exponent (int8: |log2| < 8 of a V scale, itself 1 ulp); of the sums
+    of 8 terms, 4 joins and the matrix cores' steps 24 u < 2^-19.4; together below
+    2^-18 of sum w |v|.  INT8 sums codes + 128, up to 255 / 64 of the values that count, so
+    four times that, 2^-16.  Two weights rounded to fp16 are off by up to 2^-12."""
+    print_case("weights", int8, H, KV, hd, lens)
+    g = rng(H, KV, hd, len(lens), lens[1])
+    p = Pool(g, lens, KV, hd, 16, int8)
+    for b, n in enumerate(lens):
+        pg, off = p.table[b][np.arange(n) // 16], np.arange(n) % 16
+        live = g.permutation(n)[:min(n, 8)]
+        live = live[:len(live) // 2 * 2] if n > 2 else live
+        # q has one 1 per head, in d = 0: scores are k[0], within 2^-6 of each other
+        if int8:
+            k, v = np.zeros((n, KV, hd), np.int8), np.zeros((n, KV, hd), np.int8)
+            ks = np.full((n, KV), 0.25, np.float32)
+            vs = np.full((n, KV), 0.01, np.float32)
+            k[:, :, 0] = -100
+            k[live, :, 0] = 100
+            ks[live] = 0.01 * (1 + 2.0 ** -7 * g.random((len(live), KV)))
+            v[live] = g.integers(100, 128, (1, KV, hd)).astype(np.int8)
+            v[live[::2]] *= -1
+            p.ks[pg, off], p.vs[pg, off] = ks, vs
+            p.k[b], p.v[b] = k * ks[..., None].astype(np.float64), v * vs[..., None].astype(np.float64)
+        else:
+            k, v = np.zeros((n, KV, hd), np.float16), np.zeros((n, KV, hd), np.float16)
+            k[:, :, 0] = -24
+            k[live, :, 0] = 2.0 ** -7 * g.random((len(live), KV))
+            v[live] = 1 + g.random((1, KV, hd))
+            v[live[::2]] *= -1
+            p.k[b], p.v[b] = k.astype(np.float64), v.astype(np.float64)
+        p.kp[pg, off, :, :hd], p.vp[pg, off, :, :hd] = k, v
+    p.upload()
+    q = np.zeros((len(lens), H, hd), np.float16)
+    q[..., 0] = 1.0
+    q = q.reshape(len(lens), -1)
+    got = host(attn_call(p, dev_(q), H, 1.0)).reshape(-1, H, hd).astype(np.float64)
+    for b, n in enumerate(lens):
+        want, size = attn_ref(q[b].reshape(H, hd).astype(np.float64), p.k[b], p.v[b], 1.0, 0, n)
+        tol = 2.0 ** -11 * np.abs(want) + 2.0 ** (-16 if int8 else -18) * size + 2.0 ** -25
+        err = np.abs(got[b] - want)
+        assert np.all(err <= tol), (b, n, float((err / tol).max()))
