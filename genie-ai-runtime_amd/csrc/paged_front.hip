@@ -10,7 +10,9 @@
 // is stored.  The contiguous front (qk_post_kernel, which replaces
 // decode.cu:1441-1478) keeps the reference's fp16 roundings between the steps and
 // its fp32 angle, which at position p is off by up to p * 2^-24 radians; here the
-// angle is a 64-bit fraction of a turn, exact to 2^-32 turns at every position.
+// frequency is a 64-bit fraction of a turn and the angle a 32-bit one, within 2^-31
+// turns at every position (theta >= 1): 2^-33.5 from the frequency's rounding times
+// a position below 2^31, 2^-32 from the bits that are cut off.
 //
 // Measured (32 / 8 heads x 128): 2048 tokens into INT8 pages 11.5 us (46 MB, 4.0
 // TB/s; half of it instructions), 8000 into fp16 pages 43.6 us (4.5 TB/s); 64 tokens
@@ -23,18 +25,54 @@ namespace jllm_hip {
 
 typedef uint32_t u32x2f __attribute__((ext_vector_type(2)));
 
+namespace {
+typedef unsigned __int128 u128;
+// the upper half of the 256-bit product, short by less than 4
+u128 mul_hi(u128 a, u128 b) {
+    const uint64_t a1 = (uint64_t)(a >> 64), a0 = (uint64_t)a, b1 = (uint64_t)(b >> 64), b0 = (uint64_t)b;
+    return (u128)a1 * b1 + (((u128)a1 * b0) >> 64) + (((u128)a0 * b1) >> 64);
+}
+}  // namespace
+
+// f[i] = theta^(-2 i / hd) / 2 pi, each from one before it in 128-bit fixed point and
+// rounded to 64 bits at the end: off by less than 0.51 of 2^-64 turns for theta from 1 to
+// 2^64, 0.7 above (64-bit products added up to 30 of 2^-64).  The host's time for 64 of
+// them is 0.2 us.
 void rope_turns(RopeTurns& rt, int head_dim, double theta) {
-    // theta^(-2 i / hd) / 2 pi, each from the one before it in 64-bit fixed point:
-    // off by some 2^-60 (a call of pow for each costs the host 0.9 us a launch)
-    const long double ratio = powl((long double)theta, -2.0L / head_dim);
     const int n = head_dim / 2;
-    if (ratio < 1.0L) {
-        const uint64_t r = (uint64_t)ldexpl(ratio, 64);
-        uint64_t f = 0x28BE60DB9391054Aull;                  // 2^64 / 2 pi
-        for (int i = 0; i < n; i++) {
-            rt.f[i] = f;
-            f = (uint64_t)(((unsigned __int128)f * r) >> 64);
+    if (theta > 1.0) {
+        u128 r;                                              // theta^(-1 / n)
+        if (theta < 18446744073709551616.0) {
+            // A Newton step on r^n theta = 1 from a double: the error, some 2^-50, is squared
+            // (and times n / 2).  theta = m 2^e, m a whole number of 24 bits (it is a float),
+            // so r^n m less 2^(128 - e) is 2^(128 - e) times the relative error of r^n,
+            // and fits a signed word.
+            const double ratio = pow(theta, -1.0 / n);
+            r = (u128)(uint64_t)ldexp(ratio, 64) << 64;
+            int e;
+            const uint32_t m = (uint32_t)ldexp(frexp(theta, &e), 24);
+            e -= 24;
+            u128 power = ~(u128)0, x = r;
+            for (int k = n; k > 0; k >>= 1, x = mul_hi(x, x))
+                if (k & 1) power = mul_hi(power, x);
+            const u128 one = e > 0 ? (u128)1 << (128 - e) : 0;       // modulo 2^128
+            const __int128 above = (__int128)(power * m - one);
+            r -= (u128)(__int128)(ldexp((double)above, e) * ratio / n);
+        } else {
+            // (r^n has too few bits here, but the powers of r fall so fast that 64 of r do)
+            r = (u128)(uint64_t)ldexpl(powl((long double)theta, -1.0L / n), 64) << 64;
         }
+        // four chains, so that a product need not wait for the one before it (n is a multiple of 4)
+        const u128 r2 = mul_hi(r, r), r4 = mul_hi(r2, r2);
+        u128 f[4] = {((u128)0x28BE60DB9391054Aull << 64) | 0x7F09D5F47D4D3770ull};     // 2^128 / 2 pi
+        f[1] = mul_hi(f[0], r);
+        f[2] = mul_hi(f[0], r2);
+        f[3] = mul_hi(f[1], r2);
+        for (int i = 0; i < n; i += 4)
+            for (int j = 0; j < 4; j++) {
+                rt.f[i + j] = (uint64_t)((f[j] + ((u128)1 << 63)) >> 64);
+                f[j] = mul_hi(f[j], r4);
+            }
     } else {
         for (int i = 0; i < n; i++) {
             const long double turns = powl((long double)theta, -2.0L * i / head_dim) / 6.283185307179586476925286766559L;

@@ -423,8 +423,8 @@ int jllm_hip_gemm_dense_batched(uint16_t* out, const void* W, int wtype, const u
  * k at positions[t], q to q_out, k and v into slot slots[t] of the pool: fp16,
  * or int8 codes rint(v * 127 / absmax) with the scale absmax / 127 of each
  * (slot, head).  Everything is computed in fp32 from the fp16 inputs and
- * rounded once, where it is stored; the angle is exact to 2^-32 turns at
- * every position (jllm_hip_qk_norm_rope_store_kv keeps the reference's
+ * rounded once, where it is stored; the angle is within 2^-31 turns of
+ * exact at every position for theta_base >= 1 (jllm_hip_qk_norm_rope_store_kv keeps the reference's
  * intermediate roundings and fp32 angle).  An int8 row that holds a NaN or an
  * infinity gets a NaN scale.
  * q_out, q, k, v: rows of q_out_stride, q_stride, ... halves (multiples of
