@@ -61,7 +61,10 @@ int jllm_hip_qk_norm_rope_store_kv_paged(uint16_t* q_out, int64_t q_out_stride, 
     a.q_norm = q_norm; a.k_norm = k_norm; a.k_pages = k_pages; a.v_pages = v_pages;
     a.k_scales = k_scales; a.v_scales = v_scales; a.n_slots = n_slots; a.positions = positions; a.slots = slots;
     a.n_heads = n_heads; a.n_kv = n_kv_heads; a.head_dim = head_dim; a.cache_head_dim = cache_head_dim; a.N = N;
-    a.eps = eps; a.norm_fp32 = norm_fp32 != 0; a.neox = neox != 0; a.kv_int8 = kv_int8 != 0;
+    // (the reciprocal root takes a subnormal for 0, which would make a row of zeros NaN; of
+    // other rows the mean square is above 2^-56, where neither eps is seen)
+    a.eps = eps > 0.0f && eps < 1.17549435e-38f ? 1.17549435e-38f : eps;
+    a.norm_fp32 = norm_fp32 != 0; a.neox = neox != 0; a.kv_int8 = kv_int8 != 0;
     if (paged_front_blocks(a) >= SERVING_MAX_BLOCKS) return refuse(tag, "too many tokens for one launch");
     rope_turns(a.rt, head_dim, theta_base);
     return launch_status(paged_front_launch(a, (hipStream_t)stream), tag);

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from gpu_util import print_case
-from test_serving_gpu import Pool, attn_call, attn_check, attn_ref, dev_, host, rng
+from test_serving_gpu import Pool, attn_call, attn_check, attn_ref, check_front, dev_, host, rng, run_front
 
 pytestmark = pytest.mark.gpu
 
@@ -129,3 +129,17 @@ def test_attention_weights_keep_more_than_fp16(dev, int8, H, KV, hd, lens):
         tol = 2.0 ** -11 * np.abs(want) + 2.0 ** (-16 if int8 else -18) * size + 2.0 ** -25
         err = np.abs(got[b] - want)
         assert np.all(err <= tol), (b, n, float((err / tol).max()))
+
+
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("norm", ["f32", "f16"])
+@pytest.mark.parametrize("eps", [1e-40, 1.4e-45, 1.2e-38])
+def test_front_eps_below_the_normal_range(dev, int8, norm, eps):
+    """An eps that is subnormal is an eps: rows of zeros stay zero, the others are
+    normed as if it were not there."""
+    H, KV, hd = 4, 2, 64
+    x = rng(8).standard_normal((4, (H + 2 * KV) * hd)).astype(np.float16)
+    x[1] = 0
+    x[2] = 6e-8                    # the smallest fp16
+    r = run_front(rng(9), 4, H, KV, hd, int8=int8, x=x, norm=norm, eps=eps)
+    check_front(*r, H, hd, int8)
