@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 import torch
 
+import jllm
 from gpu_util import print_case
 from test_serving_gpu import Pool, attn_call, attn_check, attn_ref, check_front, dev_, host, rng, run_front
 
@@ -143,3 +144,52 @@ def test_front_eps_below_the_normal_range(dev, int8, norm, eps):
     x[2] = 6e-8                    # the smallest fp16
     r = run_front(rng(9), 4, H, KV, hd, int8=int8, x=x, norm=norm, eps=eps)
     check_front(*r, H, hd, int8)
+
+
+# lengths of the rows at each step: over a unit's and a part's border, from several
+# pieces to one and to none and back, all short, all empty, all at max_seq
+STEPS = [[3000, 1, 0, 700, 5999, 127, 2000, 33],
+         [3001, 2, 1, 701, 6000, 128, 2001, 34],
+         [3002, 3, 0, 640, 12, 129, 0, 35],
+         [40, 6000, 5, 0, 0, 256, 6000, 1],
+         [0, 0, 0, 0, 0, 0, 0, 0],
+         [1, 0, 33, 7, 2, 100, 3, 129],
+         [6000, 6000, 6000, 6000, 6000, 6000, 6000, 6000],
+         [7000, 1, -5, 700, 5999, 127, 2000, 33]]       # (above max_seq: max_seq; below 0: empty)
+
+
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("short", [0, 62])
+def test_attention_captured_while_lengths_change(dev, int8, short):
+    """One captured call that cuts its rows, replayed while the lengths change in
+    place, its workspace holding the pieces of the steps before; and the same calls
+    eagerly on another such workspace.  Eager work and synchronizations between."""
+    print_case("captured parts", int8, short)
+    H, KV, hd, most = 8, 2, 64, 6000
+    B = len(STEPS[0]) + short
+    g = rng(90, short, int8)
+    p = Pool(g, [most] * len(STEPS[0]) + [40] * short, KV, hd, 32, int8, max_seq=most).upload()
+    q = (g.standard_normal((B, H * hd)) * 1.2).astype(np.float16)
+    Q, out = dev_(q), torch.full((B, H * hd), 7.0, dtype=torch.float16, device="cuda:0")
+    need = jllm.lib().jllm_hip_flash_attention_decode_paged_workspace(B, H, KV, hd, most, 0)
+    assert need > 0                                     # rows are cut
+    ws, ws2 = [torch.full((need,), 0xFF, dtype=torch.uint8, device="cuda:0") for _ in range(2)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        attn_call(p, Q, H, 0.125, out=out, ws=ws)       # warm-up outside the capture
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        attn_call(p, Q, H, 0.125, out=out, ws=ws)
+    for i, step in enumerate(STEPS + STEPS[::-1]):
+        lens = step + [(i + j) % 41 for j in range(short)]
+        p.d[5].copy_(dev_(np.array(lens, np.int32)))
+        out.fill_(7.0)
+        gr.replay()
+        got = host(out).copy()
+        attn_check(p, got, q, H, 0.125, lens=[min(n, most) for n in lens])
+        torch.ones(1000, device="cuda:0").cumsum(0)
+        eager = host(attn_call(p, Q, H, 0.125, ws=ws2))
+        assert np.array_equal(got.view(np.uint16), eager.view(np.uint16)), i
