@@ -280,8 +280,9 @@ void paged_attn_kernel(PagedAttnArgs a, PagedPlan plan) {
         return x;
     };
 
-    // (zeroed: where a path leaves such registers undefined, this compiler has
-    // given words of a loaded row to other values while they were still needed)
+    // (zeroed: some dozen instructions a wave, so that no path has them undefined.  The
+    // listings show no need: with and without, no word of a loaded row is written
+    // before it is read in the loop.)
     u32x4a rk[2][KC > 0 ? KC : 1] = {};
     u32x2a rt[2] = {};
     uint32_t rv[8][VW] = {};
@@ -645,9 +646,10 @@ namespace {
 // against 9.8, of 600 9.7 against 8.8, of 1000 13.2 against 9.0; 16 rows of 700 13.1
 // against 15.2; 64 of 1000 54 against 60; 256 of 700 INT8 77 against 100; 8 of 1500 20.5
 // against 15.4).
-// Also for more rows than PA_MAX_ROWS, which fill the card by themselves: 1500 rows up
-// to 2000 of 4 / 1 heads x 32 29 us whole, 38 cut; 1500 INT8 rows of 1100 of 16 / 2
-// heads 161 against 189, though 1100 fp16 rows up to 1200 101 against 84.
+// Also for more rows than PA_MAX_ROWS: that is as far as a workgroup counts through all
+// lengths, no gain.  1500 rows up to 2000 of 4 / 1 heads x 32 29 us whole, 38 cut, and 1500
+// INT8 rows of 1100 of 16 / 2 heads 161 against 189, but 1100 fp16 rows up to 1200 101
+// against 84, and one long row among them is a single workgroup's, 8 us for 1000 keys.
 // Parts: as many as the card holds at once, three workgroups on each of 256 CUs.
 // Heads per workgroup: KV heads that run side by side read neighbouring pieces of the
 // same rows.  Pieces under 128 bytes share their lines (all lengths drawn; one head

@@ -424,15 +424,17 @@ int jllm_hip_gemm_dense_batched(uint16_t* out, const void* W, int wtype, const u
  * or int8 codes rint(v * 127 / absmax) with the scale absmax / 127 of each
  * (slot, head).  Everything is computed in fp32 from the fp16 inputs and
  * rounded once, where it is stored; the angle is within 2^-31 turns of
- * exact at every position for theta_base >= 1 (jllm_hip_qk_norm_rope_store_kv keeps the reference's
- * intermediate roundings and fp32 angle).  An int8 row that holds a NaN or an
- * infinity gets a NaN scale.
+ * exact at every position for theta_base >= 1
+ * (jllm_hip_qk_norm_rope_store_kv keeps the reference's intermediate roundings
+ * and fp32 angle).  An int8 row that holds a NaN or an infinity gets a NaN
+ * scale, a row of zeros the scale 0.
  * q_out, q, k, v: rows of q_out_stride, q_stride, ... halves (multiples of
  * 4: slices of a fused QKV buffer will do), 8-byte aligned; q_out may be q
  * itself, otherwise its rows overlap none of the inputs'.
  * A token whose slot is outside [0, n_slots) is padding: its q_out row and
  * the pool are left as they are.  The slots of one call must be distinct.
- * head_dim a multiple of 8 up to 128; pages 16-byte aligned, cache rows a
+ * head_dim a multiple of 8 up to 128 (jllm_hip_flash_attention_decode_paged
+ * reads multiples of 32 only); pages 16-byte aligned, cache rows a
  * multiple of 16 bytes.  neox and norm_fp32 as jllm_hip_qk_norm_rope_store_kv. */
 int jllm_hip_qk_norm_rope_store_kv_paged(uint16_t* q_out, int64_t q_out_stride, const uint16_t* q, int64_t q_stride,
                                          const uint16_t* k, int64_t k_stride, const uint16_t* v, int64_t v_stride,
@@ -446,23 +448,31 @@ int jllm_hip_qk_norm_rope_store_kv_paged(uint16_t* q_out, int64_t q_out_stride, 
  * attends to positions [0, seq_lens[b]) (the last `window` of them when
  * window > 0) of block_table row b, i.e. block_table + b * table_stride.
  * q rows of q_stride halves (a multiple of 8), out [B][n_heads * head_dim]
- * fp16, not overlapping q.  A row of length <= 0 gives zeros; a length above max_seq counts as
- * max_seq (host: the longest a row can be; it sizes the split of the keys).
+ * fp16, not overlapping q.  Scores, softmax and sums are fp32, with the weights
+ * held to 2^-21 for the product with V; the output is rounded to fp16 once.
+ * A row of length <= 0 gives zeros, as does one whose scores are all -inf;
+ * a length above max_seq counts as max_seq (host: the longest a row can be; it
+ * sizes the split of the keys).
  * The keys of a page id outside [0, n_pages) are skipped.  Slots of a page
  * behind the end of its sequence may hold anything.  Several query tokens
  * of one sequence (a prompt chunk) are passed as one row each, with the same
- * table row and growing lengths.
+ * table row and growing lengths; each of them reads its keys for itself.
  * The keys are dealt out to workgroups by the lengths of all rows, so a
  * row's result can differ in its last bits with the rows beside it; the same
  * call gives the same bits.  JLLM_SPLITK=0 in the environment (read once)
  * leaves every row whole: slower where rows are few and long, and without
- * a workspace.
+ * a workspace.  So are the rows of a call with more than 1024 of them, and a
+ * long one among those keeps one workgroup busy while the others are done:
+ * give long rows in calls of up to 1024.
  * page_size a power of two from 16 to 4096; head_dim, heads and KV types
  * as in jllm_hip_flash_attention_decode, n_heads and cache_head_dim <= 4096
- * (scales NULL = 1.0).
+ * (scales NULL = 1.0; an infinite or NaN scale of a V row makes its KV head's
+ * outputs NaN).
  * workspace: 16-byte aligned, any content, at least the bytes that
  * jllm_hip_flash_attention_decode_paged_workspace says, which returns a
- * negative JLLM_ERR_* for sizes that the operator refuses. */
+ * negative JLLM_ERR_* for sizes that the operator refuses.  The bytes do not
+ * grow with B or max_seq everywhere (rows that are left whole need none): a
+ * workspace for calls of several sizes is as large as the largest of theirs. */
 int64_t jllm_hip_flash_attention_decode_paged_workspace(int B, int n_heads, int n_kv_heads, int head_dim, int max_seq,
                                                         int window);
 int jllm_hip_flash_attention_decode_paged(uint16_t* out, const uint16_t* q, int64_t q_stride, const void* k_pages,
@@ -492,7 +502,8 @@ int jllm_hip_flash_attention_decode_paged(uint16_t* out, const uint16_t* q, int6
  * none is finite (a mask that leaves nothing); jllm_hip_dequant_embedding_rows
  * reads -1 as a zero row.
  * workspace (for next_token only): 8-byte aligned, at least the bytes that
- * jllm_hip_logits_process_workspace says. */
+ * jllm_hip_logits_process_workspace says; these do not grow with B and V
+ * everywhere either. */
 int64_t jllm_hip_logits_process_workspace(int B, int V);
 int jllm_hip_logits_process(float* out, int64_t out_stride, const float* logits, int64_t logits_stride, int B, int V,
                             const int32_t* tokens, int64_t token_stride, const int32_t* n_prompt,
