@@ -23,7 +23,7 @@
 //                 the 128 leaves through the accumulator's start value for K, and through
 //                 the sum of the weights for V).
 // Sums, maxima and accumulators are fp32.  For the matrix cores a weight is split into
-// two fp16 parts, each rounded down, as in the other attention kernels: together 2^-21
+// two fp16 parts, as in the other attention kernels: together within 2^-21
 // of the weight, so the output's rounding is the only one to 11 bits (with one part,
 // 2^-12 of sum w |v|, values that cancel lost their difference).  The second product
 // and the split cost 0.3 % of 24 fp16 rows of up to 16384, 1.5 % of 48 INT8 rows of up
@@ -467,15 +467,19 @@ void paged_attn_kernel(PagedAttnArgs a, PagedPlan plan) {
             for (int j = 0; j < NT; j++) acc[j] *= corr;
             if (INT8) wsum *= corr;
         }
-        h8 pb, pl;                                     // p * PA_LIFT in two parts, each rounded down
+        // p * PA_LIFT in two parts, each rounded down.  fp16 V may be infinite, and 0 * inf
+        // is no part of inf: there the low part of a weight that is not 0 gets its last bit.
+        u32x4a hw, lw;
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
             const float x = p[e] * PA_LIFT, y = p[e + 1] * PA_LIFT;
             const auto hi = __builtin_amdgcn_cvt_pkrtz(x, y);
             const auto lo = __builtin_amdgcn_cvt_pkrtz(x - (float)hi[0], y - (float)hi[1]);
-            pb[e] = (_Float16)hi[0]; pb[e + 1] = (_Float16)hi[1];
-            pl[e] = (_Float16)lo[0]; pl[e + 1] = (_Float16)lo[1];
+            const uint32_t h = __builtin_bit_cast(uint32_t, hi);       // (no sign bits)
+            hw[e / 2] = h;
+            lw[e / 2] = __builtin_bit_cast(uint32_t, lo) | (INT8 ? 0u : (h + 0x7FFF7FFFu) >> 15 & 0x00010001u);
         }
+        const h8 pb = __builtin_bit_cast(h8, hw), pl = __builtin_bit_cast(h8, lw);
         // 3. O^T += V^T P^T
         if (!INT8 && !full) {                          // what a slot without a key holds may be NaN
 #pragma unroll

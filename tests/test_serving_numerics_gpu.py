@@ -193,3 +193,27 @@ def test_attention_captured_while_lengths_change(dev, int8, short):
         torch.ones(1000, device="cuda:0").cumsum(0)
         eager = host(attn_call(p, Q, H, 0.125, ws=ws2))
         assert np.array_equal(got.view(np.uint16), eager.view(np.uint16)), i
+
+
+@pytest.mark.parametrize("lens", [[1, 2, 40, 300], [3000, 1, 17]])
+@pytest.mark.parametrize("bad", [np.inf, -np.inf])
+def test_attention_infinite_values_of_any_weight(dev, bad, lens):
+    """An infinite V value of a key that has a weight makes its own dimension
+    infinite, whatever the weight (1, equal shares, 2^-30 of the others), and no other."""
+    print_case("infinite values", bad, lens)
+    H, KV, hd = 8, 2, 64
+    for s_low in (0.0, -20.0):                    # the key's score; the others' are 0
+        p = Pool(rng(len(lens), 70), lens, KV, hd, 16, False)
+        for b, n in enumerate(lens):
+            pg, off = p.table[b][np.arange(n) // 16], np.arange(n) % 16
+            p.kp[pg, off, :, :hd] = 0
+            t = n // 2
+            p.kp[pg[t], off[t], :, 0] = s_low
+            p.vp[pg[t], off[t], 1, 5] = bad
+        p.upload()
+        q = np.zeros((len(lens), H, hd), np.float16)
+        q[..., 0] = 1
+        got = host(attn_call(p, dev_(q.reshape(len(lens), -1)), H, 1.0)).reshape(-1, H, hd)
+        want = np.zeros(got.shape, bool)
+        want[:, H // 2:, 5] = True
+        assert np.all(got[want] == bad) and np.isfinite(got[~want]).all()
