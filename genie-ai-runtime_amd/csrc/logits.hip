@@ -8,8 +8,9 @@
 //   y = -inf                     where the token's mask bit is 0
 //   token = lowest index of the largest finite y, -1 when there is none
 //
-// Measured (both launches): 64 rows x 151936 with up to 4096 listed tokens, biases and
-// masks 20.0 us (4.0 TB/s), without any 15.3; 251 rows x 32003 17.1 us; one row 5.6 us.
+// Measured (both launches, replayed): 64 rows x 151936 with up to 4096 listed tokens,
+// biases and masks 20.0 us (4.0 TB/s), without any 15.3; 251 rows x 32003 17.0 us; one
+// row 5.8 us, of which the kernels run 4.0 and 1.9 (7.9 us where the host launches them).
 #include "kq_common.h"
 #include "serving.h"
 
@@ -202,7 +203,8 @@ __global__ __launch_bounds__(LG_THREADS) void logits_pick_kernel(int32_t* tok, c
 namespace {
 // Parts of 2048 tokens, which search the lists half as often, once they fill the
 // card, else of 1024 (one row of 151936 with 700 tokens listed: 5.8 us against 7.1 with
-// parts of 4096; 64 rows with lists, biases and masks: 22.3 us, 24.6 with 4096).
+// parts of 4096; 64 rows with lists, biases and masks, when they took 22.3 us: 24.6 with
+// 4096).
 int logits_part(int B, int V) { return (int64_t)B * (((int64_t)V + 2047) / 2048) < 1024 ? 1 : 2; }
 int logits_chunks(int B, int V) {
     const int ch = 1024 * logits_part(B, V);

@@ -26,7 +26,7 @@
 // two fp16 parts, as in the other attention kernels: together within 2^-21
 // of the weight, so the output's rounding is the only one to 11 bits (with one part,
 // 2^-12 of sum w |v|, values that cancel lost their difference).  The second product
-// and the split cost 0.3 % of 24 fp16 rows of up to 16384, 1.5 % of 48 INT8 rows of up
+// and the split cost 0.5 % of 24 fp16 rows of up to 16384, 1.5 % of 48 INT8 rows of up
 // to 4096 and at most 2.5 % (64 INT8 rows of 4 / 1 heads x 32, 15.2 us).  The parts are
 // of the weight times 2^14, so that they become subnormal only below 2^-28 of the largest.
 // With int8 the V scales go into the exponent, e^(s_t - m) vs_t = 2^(s'_t + log2
@@ -34,9 +34,9 @@
 // fp32 sums neither) or swamps the others, and a scale of 0 is a weight of 0.
 //
 // Measured (32 / 8 heads x 128, both launches): 131072 fp16 keys of one row 92 us and
-// 24 rows of up to 16384 102 us (5.8 TB/s: the reads are the bound), 48 INT8 rows of
-// up to 4096 38.9 us (3.8 TB/s; start, join and the scales' lines are the rest), one
-// INT8 row of 700 9.1 us.
+// 24 rows of up to 16384 103 us (5.8 TB/s: the reads are the bound), 48 INT8 rows of
+// up to 4096 39.8 us (3.8 TB/s; start, join and the scales' lines are the rest), one
+// INT8 row of 700 9.3 us.
 #include "attention.h"
 #include "attn_common.h"
 #include "serving.h"
