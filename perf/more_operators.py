@@ -156,7 +156,7 @@ def _prepare_norms(c, seed):
     if c["codes"]:
         s.codes = torch.zeros((rows, hidden), dtype=torch.int8, device=DEV)
         s.scales = torch.zeros((rows,), device=DEV)
-        s.values = torch.zeros((rows, hidden), dtype=torch.float16, device=DEV)
+        s.values = torch.zeros((rows, hidden), device=DEV)
     else:
         s.y = torch.zeros((rows, hidden), dtype=torch.float16, device=DEV)
     return s
