@@ -28,6 +28,7 @@
 // the product and added to the columns that see it.
 #include <type_traits>
 #include "paged_common.h"
+#include "prefix_window.h"
 
 namespace jllm_hip {
 
@@ -105,7 +106,7 @@ void paged_prefix_kernel(PagedAttnArgs a, PagedPrefixArgs pre) {
         int lo = len;
         for (int b = (int)threadIdx.x; b < a.B; b += 64 * PA_WAVES) {
             const int n = min(a.lens[b], a.max_seq);
-            if (n >= 0) lo = min(lo, (int)max((int64_t)len + n - a.window, (int64_t)0));
+            if (n >= 0) lo = min(lo, first_seen(len, n, a.window));
         }
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) lo = min(lo, __shfl_xor(lo, o, 64));
@@ -133,9 +134,9 @@ void paged_prefix_kernel(PagedAttnArgs a, PagedPrefixArgs pre) {
         dead[j] = !is;
         if (WINDOW) {
             const int n = min(a.lens[b], a.max_seq);
-            const int64_t first = (int64_t)len + n - a.window;
+            const int first = first_seen(len, n, a.window);
             dead[j] = dead[j] || n < 0 || first >= len;
-            lo[j] = dead[j] || first < 0 ? 0 : (int)first;
+            lo[j] = dead[j] ? 0 : first;
         }
         lo_max = max(lo_max, lo[j]);
 #pragma unroll
@@ -631,7 +632,7 @@ void prefix_tile_kernel(PagedAttnArgs a, PagedPrefixArgs pre) {
         int lo = len;
         for (int b = tid; b < a.B; b += 64 * PT_WAVES) {
             const int n = min(a.lens[b], a.max_seq);
-            if (n >= 0) lo = min(lo, (int)max((int64_t)len + n - a.window, (int64_t)0));
+            if (n >= 0) lo = min(lo, first_seen(len, n, a.window));
         }
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) lo = min(lo, __shfl_xor(lo, o, 64));
@@ -755,9 +756,9 @@ void prefix_tile_kernel(PagedAttnArgs a, PagedPrefixArgs pre) {
         dead[j] = !is;
         if (WINDOW) {
             const int n = min(a.lens[b], a.max_seq);
-            const int64_t first = (int64_t)len + n - a.window;
+            const int first = first_seen(len, n, a.window);
             dead[j] = dead[j] || n < 0 || first >= len;
-            lo[j] = dead[j] || first < 0 ? 0 : (int)first;
+            lo[j] = dead[j] ? 0 : first;
         }
         lo_max = max(lo_max, lo[j]);
 #pragma unroll
