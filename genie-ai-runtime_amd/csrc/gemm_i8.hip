@@ -21,9 +21,15 @@ typedef __attribute__((address_space(3))) void lds_void_g;
 
 namespace {
 
+// Every form rounds alike, the product before the bias is added (a fused multiply and add
+// where the compiler sees both would give a token other bits among many than among few).
+__device__ __forceinline__ float scaled_by(int sum, float xs, float ws, bool biased, float bias) {
+#pragma clang fp contract(off)
+    const float v = (float)sum * xs * ws;
+    return biased ? v + bias : v;
+}
 __device__ __forceinline__ float scaled(const GemmI8Args& a, int sum, float xs, int m) {
-    const float v = (float)sum * xs * a.ws[m];
-    return a.bias ? v + a.bias[m] : v;
+    return scaled_by(sum, xs, a.ws[m], a.bias != nullptr, a.bias ? a.bias[m] : 0.0f);
 }
 __device__ __forceinline__ void store1(const GemmI8Args& a, int n, int m, float v) {
     const int64_t at = (int64_t)n * a.y_stride + m;
@@ -291,10 +297,7 @@ __device__ __forceinline__ void tile_body(const GemmI8Args& a, uint8_t* tiles, i
                 const f32x4g ws = *(const f32x4g*)(sw_ + m), bias = *(const f32x4g*)(sb_ + m);
                 f32x4g y;
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    y[r] = (float)sum[r] * xs * ws[r];
-                    if (a.bias) y[r] += bias[r];
-                }
+                for (int r = 0; r < 4; r++) y[r] = scaled_by(sum[r], xs, ws[r], a.bias != nullptr, bias[r]);
                 if (half) *(u32x2g*)(to + 2 * m) = u32x2g{(uint32_t)f32_to_f16_bits(y[0]) | (uint32_t)f32_to_f16_bits(y[1]) << 16,
                                                           (uint32_t)f32_to_f16_bits(y[2]) | (uint32_t)f32_to_f16_bits(y[3]) << 16};
                 else      *(f32x4g*)(to + 4 * m) = y;

@@ -578,8 +578,9 @@ int jllm_hip_block_norms(void* h, int64_t h_stride, const void* residual, int64_
  *   y[n][m] = x_scales[n] * w_scales[m] * sum_k x[n][k] W[m][k] (+ bias[m])
  * for N tokens, M channels; x and W int8 rows of K codes (-128 allowed), y fp32
  * rows when y_fp32, else fp16, bias fp32 or NULL.  The sums are exact in int32;
- * the fp32 result is ((sum * x_scale) * w_scale) + bias, and rounded once more to
- * fp16.  Codes and scales are those of jllm_hip_block_norms, or of the row
+ * the fp32 result is ((sum * x_scale) * w_scale) + bias with the sum and every
+ * step rounded to fp32, and rounded once more to fp16: a token's outputs are the
+ * same bits whatever tokens are beside it.  Codes and scales are those of jllm_hip_block_norms, or of the row
  * quantiser jllm_hip_fp16_to_int8, for weights with channels as its rows.
  * K a multiple of 16 up to 131056; x_stride and w_stride bytes, multiples of 16,
  * y_stride elements; x and W 16-byte aligned, in device memory; y overlaps no
