@@ -171,8 +171,37 @@ __global__ __launch_bounds__(T) void block_norms_kernel(BlockNormsArgs a) {
         }
     }
     if (a.codes) {
-        const float m = __builtin_bit_cast(float, top), scale = f * m * (1.0f / 127.0f);
-        const bool fine = scale <= 3.402823466e+38f;    // a row with an infinity or NaN has no scale
+        float m = __builtin_bit_cast(float, top), by = 1.0f, scale;
+        const bool far = !(m >= 0x1p-100f && m <= 0x1p126f);
+        if (far) by = f;
+#pragma unroll
+        for (int i = 0; i < E; i++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) r[i][e] *= v[i][e] * by;
+        scale = f * m * (1.0f / 127.0f);
+        if (far) {
+            // h times the weights has left fp32's range, or is about to, where y need not: the
+            // codes are y's own then, by a maximum of their own.  (Rows of zeros, infinities and
+            // NaN come here too.)
+            top = 0;
+#pragma unroll
+            for (int i = 0; i < E; i++)
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    if (t + i * T < pieces) top = max(top, __builtin_bit_cast(uint32_t, r[i][e]) & 0x7FFFFFFFu);
+            top = wave_max_u32(top);
+            if (W > 1) {
+                __syncthreads();                       // (the first maximum has been read)
+                if (lane == 0) sTop[wave] = top;
+                __syncthreads();
+                top = 0;
+#pragma unroll
+                for (int w = 0; w < W; w++) top = max(top, sTop[w]);
+            }
+            m = __builtin_bit_cast(float, top);
+            scale = m * (1.0f / 127.0f);
+        }
+        const bool fine = m <= 3.402823466e+38f && scale <= 3.402823466e+38f;   // a row with an infinity or NaN has no scale
         // (magnitudes under 2^-100: 127 / m might be infinite)
         const float lift = m < 0x1p-100f ? 0x1p96f : 1.0f, ml = m * lift;
         const float inv = ml > 0.0f ? 127.0f / ml : 0.0f;
@@ -184,7 +213,7 @@ __global__ __launch_bounds__(T) void block_norms_kernel(BlockNormsArgs a) {
             u32x2n o = {0u, 0u};
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const float q = fminf(fmaxf(__builtin_rintf(v[i][e] * r[i][e] * lift * inv), -127.0f), 127.0f);
+                const float q = fminf(fmaxf(__builtin_rintf(r[i][e] * lift * inv), -127.0f), 127.0f);
                 o[e / 4] |= (uint32_t)((int)(fine ? q : 0.0f) & 0xFF) << (8 * (e % 4));
             }
             *(u32x2n*)(a.codes + row * a.code_stride + 8 * p) = o;

@@ -560,10 +560,11 @@ int jllm_hip_logits_process(float* out, int64_t out_stride, const float* logits,
  * and pre_norm: hidden_dim values, fp32 when norm_fp32, else fp16; pre_norm may
  * be NULL when neither y nor codes are asked for.  At least one output.
  * Everything is computed in fp32 and rounded once, where it is stored: y is
- * formed from h before its rounding.  Squares are summed in fp32: magnitudes
- * of x and h under 2^56 (and, where eps is 0, a row's largest above 2^-56: a row
- * of zeros is then NaN).  A row of codes whose y holds an infinity or NaN has
- * codes 0 and the scale NaN, a row of zeros codes and scale 0.
+ * formed from h before its rounding.  Squares are summed in fp32: magnitudes of
+ * x, t and h under 2^56 and, where eps is under 2^-100, a row's largest above
+ * 2^-56 (with an eps of 0 a row of zeros is NaN); pre_norm may be of any size.
+ * A row of codes whose y holds an infinity or NaN has codes 0 and the scale NaN,
+ * a row of zeros codes and scale 0.
  * Strides in elements, at least hidden_dim and multiples of 16 bytes (codes:
  * of 8); pointers 16-byte aligned (codes 8, code_scales 4).  hidden_dim a multiple
  * of 8 up to 32768, rows < 2^22.  h may be residual itself and y may be x itself
