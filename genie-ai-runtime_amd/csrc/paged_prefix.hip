@@ -710,9 +710,10 @@ void prefix_tile_kernel(PagedAttnArgs a, PagedPrefixArgs pre) {
             vsr = a.vs ? a.vs[at] : 1.0f;
         }
     };
-    // the scale's sign goes into q, so that the largest product is the largest score; a scale
-    // of 0 is one that no finite product brings near 1
-    const float f0 = fmaxf(fabsf(a.scale) * PA_LOG2E, 1e-30f);
+    // the scale's sign goes into q, so that the largest product is the largest score; with fp16
+    // keys a scale of 0 is one that no finite product brings near 1 (masked products are -inf
+    // before they meet it; those of INT8 keys, which may have any scale, after)
+    const float f0 = fmaxf(fabsf(a.scale) * PA_LOG2E, INT8 ? 0.0f : 1e-30f);
     auto put = [&](int s) {                                       // the fetched stage into LDS
         uint8_t* st = ring + (s & 1) * 2 * HALF;
         const int tid_ = anew(tid);
