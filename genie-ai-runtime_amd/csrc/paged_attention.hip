@@ -345,7 +345,7 @@ void paged_attn_kernel(PagedAttnArgs a, PagedPlan plan) {
         for (int st = 0; st < NST; st++) start = __builtin_amdgcn_mfma_f32_16x16x32_f16(off, qb[st], start, 0, 0, 0);
         start = -start;
     }
-    const float f0 = a.scale * PA_LOG2E, f8 = f0 * 16777216.0f;
+    const float f0 = a.scale * PA_LOG2E;
 
     float m = -INFINITY, L = 0.0f, M = -INFINITY;      // maximum, this lane's sum; maximum with the V scales
     f32x4p acc[NT], wsum = {};
@@ -385,7 +385,7 @@ void paged_attn_kernel(PagedAttnArgs a, PagedPlan plan) {
         __builtin_amdgcn_sched_barrier(0);
         float sv = 0.0f;
         if (INT8) {
-            sv = li < 8 ? sraw * f8 : __builtin_amdgcn_logf(fabsf(sraw));
+            sv = li < 8 ? sraw * f0 * 16777216.0f : __builtin_amdgcn_logf(fabsf(sraw));
             s[0] *= row_bcast<0>(sv); s[1] *= row_bcast<1>(sv); s[2] *= row_bcast<2>(sv); s[3] *= row_bcast<3>(sv);
             s[4] *= row_bcast<4>(sv); s[5] *= row_bcast<5>(sv); s[6] *= row_bcast<6>(sv); s[7] *= row_bcast<7>(sv);
         } else {

@@ -273,7 +273,7 @@ void paged_prefix_kernel(PagedAttnArgs a, PagedPrefixArgs pre) {
             start[j] = -start[j];
         }
     }
-    const float f0 = a.scale * PA_LOG2E, f8 = f0 * 16777216.0f;
+    const float f0 = a.scale * PA_LOG2E;
 
     float m[NR], L[NR], M[NR];                         // maximum, this lane's sum; maximum with the V scales
     f32x4p acc[NR][NT], wsum[NR];
@@ -321,7 +321,7 @@ void paged_prefix_kernel(PagedAttnArgs a, PagedPrefixArgs pre) {
         const Tile next = next_tile();
         if (next.p0 >= 0) load_k(next.s0, next.s1);
         // lanes li < 8: the K factor, li >= 8: log2 of the V scale
-        const float sv = INT8 ? (li < 8 ? sraw * f8 : __builtin_amdgcn_logf(fabsf(sraw))) : 0.0f;
+        const float sv = INT8 ? (li < 8 ? sraw * f0 * 16777216.0f : __builtin_amdgcn_logf(fabsf(sraw))) : 0.0f;
         float kf[8], vf[8];
         if (INT8) {
             kf[0] = row_bcast<0>(sv); kf[1] = row_bcast<1>(sv); kf[2] = row_bcast<2>(sv); kf[3] = row_bcast<3>(sv);

@@ -24,3 +24,17 @@ def test_prefix_scale_and_k_scales_far_from_one(dev, power, window, B, G):
     p.upload()
     far = host(call(p, dev_(q), G, 0.125 * 2.0 ** power, window))
     assert np.array_equal(near.view(np.uint16), far.view(np.uint16))
+
+
+@pytest.mark.parametrize("B,G", COLUMNS)
+def test_prefix_largest_scales(dev, B, G):
+    """A scale that is finite, but not with the 2^24 that a form's codes carry."""
+    print_case("prefix largest scales", B, G)
+    g = rng(B, G)
+    p = pool(g, 333, [0, 7, 40] + [3] * (B - 3), 1, 64, 16, True).upload()
+    q = queries(g, B, G, 64)
+    near = host(call(p, dev_(q), G, 0.125))
+    p.ks *= np.float32(2.0 ** -112)
+    p.upload()
+    far = host(call(p, dev_(q), G, 2.0 ** 109))
+    assert np.array_equal(near.view(np.uint16), far.view(np.uint16))
