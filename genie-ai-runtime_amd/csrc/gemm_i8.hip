@@ -8,6 +8,7 @@
 // how fast a CU has them (2560 x 9728 9.5 us); to about 256 the rate at which a CU reads; beyond, the
 // matrix cores and the clock that their power leaves (8192^3 482 us, 2.28 POP/s, at 1.9 GHz,
 // of whose cycles they are busy 56 %; the rest is the waits at a stage's barrier).
+#include "gemm_i8_plan.h"
 #include "kq_common.h"
 #include "serving.h"
 
@@ -178,7 +179,6 @@ __device__ __forceinline__ void put_rows(const uint8_t* lds, int pitch, uint8_t*
 // LDS, the next one on its way while one is worked on.  Piece c (16 bytes) of row r lies
 // at place c ^ (r / 2 % 8): two rows fill the 64 banks, and the same piece of any 16 rows that
 // a read takes at once falls on each of them once.
-constexpr int GT_K = 128;
 
 // 16 bytes a lane from base + offset straight to LDS, lane after lane
 __device__ __forceinline__ void load_lds(__amdgpu_buffer_rsrc_t base, uint8_t* lds, int offset) {
@@ -402,61 +402,6 @@ __global__ __launch_bounds__(256) void gemm_i8_far_kernel(GemmI8Args a) {
     }
 }
 
-// How the product is cut.  What a stage of 128 codes costs a CU with one tile of a kind at
-// work and with as many as fit, and what a tile costs beside its stages, in us (64 stages
-// or 16, half a round of tiles to twelve):
-//   256 x 256            1.71       + 10.3     (8192^3 481; 568 with 128 x 256, 560 with 128 x 128)
-//   128 x 256            0.86, 1.0  +  6.3     (32003 channels, 251 tokens 38.6; 45 with 128 x 128)
-//   128 x 128, two       0.86, 0.98 +  3.5, 7
-//   64 x 64, two         0.28, 0.49 +  3       (4096 x 4096, 256 tokens 14.6; 21 with 128 x 128)
-//   32 x 64, up to three 0.24, 0.55 +  2.5     (6144 x 2560, 64 tokens 9.5; 11 with 64 x 64)
-// The first is bound by the matrix cores at the clock that their power leaves, the
-// others by the 57 GB/s at which one CU reads.  Sums of parts: 4 us and their bytes twice at
-// 6 TB/s (2560 x 9728, 64 tokens in 6 parts 14.1; 26 in one).  The plan is what these say
-// takes least.
-// Few tokens: channels from which a wave has 16 pieces on the way; codes from which 16 waves
-// share K, where there is no more than a workgroup for each CU (4096 x 28672, one token 25.1 us,
-// 28.0 with four; 8192 x 9728 18.2 and 17.5).
-constexpr int FEW_MANY_CHANNELS = 16384, FEW_LONG_K = 8192, FEW_CHANNELS = 4096;
-struct GemmPlan { int few, tile, splits, whole; };
-struct TileKind { int tm, tn, share; float alone, full, tile, tiles; };
-constexpr TileKind TILES[] = {{256, 256, 1, 1.71f, 1.71f, 10.3f, 10.3f}, {128, 256, 1, 0.93f, 0.93f, 6.3f, 6.3f}, {128, 128, 2, 0.86f, 0.98f, 3.5f, 7.0f},
-                              {64, 64, 2, 0.28f, 0.49f, 3.0f, 3.3f}, {32, 64, 3, 0.24f, 0.55f, 2.5f, 3.0f}};
-GemmPlan gemm_plan(int M, int N, int K) {
-    GemmPlan best = {};
-    best.splits = 1;
-    if (N <= 16) {
-        best.few = 1;
-        return best;
-    }
-    float least = 1e30f;
-    const int stages = (K + GT_K - 1) / GT_K;
-    for (int k = 0; k < 5; k++) {
-        const TileKind& t = TILES[k];
-        const int64_t n = (((int64_t)M + t.tm - 1) / t.tm) * (((int64_t)N + t.tn - 1) / t.tn), room = 256 * t.share;
-        for (int s = 1; s <= 16; s++) {
-            if (s > 1 && (s * 4 > stages || n * s > room)) break;
-            const float st = (float)((stages + s - 1) / s);
-            const int64_t wgs = n * s, rest = wgs % room;
-            float us = (float)(wgs / room) * (st * t.full + t.tiles);
-            int whole = 0;
-            if (k == 0 && s == 1 && n > room && rest > 0 && rest <= room / 2) {
-                whole = (int)(n - rest);               // the rest as halves
-                us += st * 1.05f + 6.5f;
-            } else if (rest > 0) {
-                const float f = t.share > 1 ? (float)((rest - 1) / 256) / (float)(t.share - 1) : 0.0f;
-                us += st * (t.alone + f * (t.full - t.alone)) + t.tile + f * (t.tiles - t.tile);
-            }
-            if (s > 1) us += 4.0f + (float)s * (float)M * (float)N * (8.0f / 6e6f);
-            if (us < least) {
-                least = us;
-                best.tile = k; best.splits = s; best.whole = whole;
-            }
-        }
-    }
-    return best;
-}
-
 template <int FM, int FN, int WM, int WN, int R>
 constexpr int tile_lds() {
     constexpr int TM = 32 * FM * WM, TN = 32 * FN * WN, MAIN = R * (TM + TN) * GT_K, OUT = 32 * WN * (TM * 4 + 16) + 8 * TM;
@@ -491,8 +436,8 @@ hipError_t gemm_i8_launch(const GemmI8Args& a, hipStream_t st) {
     const GemmPlan p = gemm_plan(a.M, a.N, a.K);
     if (p.few) {
         const dim3 grid((unsigned)(a.M + 15) / 16);
-        if (a.M >= FEW_MANY_CHANNELS) hipLaunchKernelGGL((gemm_i8_few_kernel<4, 8>), grid, dim3(256), 0, st, a);
-        else if (a.K >= FEW_LONG_K && a.M <= FEW_CHANNELS) hipLaunchKernelGGL((gemm_i8_few_kernel<16, 5>), grid, dim3(1024), 0, st, a);
+        if (p.few == FEW_MANY_CHANNELS) hipLaunchKernelGGL((gemm_i8_few_kernel<4, 8>), grid, dim3(256), 0, st, a);
+        else if (p.few == FEW_LONG_K) hipLaunchKernelGGL((gemm_i8_few_kernel<16, 5>), grid, dim3(1024), 0, st, a);
         else hipLaunchKernelGGL((gemm_i8_few_kernel<4, 5>), grid, dim3(256), 0, st, a);
         return hipGetLastError();
     }
