@@ -6,7 +6,7 @@ import torch
 
 import jllm
 from gpu_util import print_case
-from test_paged_prefix_gpu import queries
+from test_paged_prefix_gpu import call, pool, queries, reference
 from test_serving_gpu import attn_ref, dev_, host, rng
 
 pytestmark = pytest.mark.gpu
@@ -57,3 +57,19 @@ def test_prefix_and_own_tokens_past_31_bits_in_a_window(dev, int8, B, G, P, long
         want, size = attn_ref(q[b].reshape(G, hd).astype(np.float64), k64[at], v64[at], float(np.float32(0.1)), 0, window)
         tol = 2.0 ** -11 * np.abs(want) + 2.0 ** -10 * size + 2.0 ** -25
         assert np.all(np.abs(got[b] - want) <= tol), (b, float((np.abs(got[b] - want) / tol).max()))
+
+
+@pytest.mark.parametrize("scale", [-0.09, 2.0])
+@pytest.mark.parametrize("B,G", [(20, 4), (17, 8), (40, 16)])
+def test_prefix_int8_codes_through_lds_are_exact(dev, scale, B, G):
+    """Of more than 64 columns the prefix's INT8 codes meet the weights as they are, without the
+    128 that the form for few columns adds and takes off: what that may leave, 2 n 2^-24 255
+    max |vs| over n keys, remains for a row's own 7 keys alone."""
+    print_case("prefix exact codes", scale, B, G)
+    g = rng(B, G, 9)
+    p = pool(g, 333, [7] * B, 1, 64, 16, True).upload()
+    q = queries(g, B, G, 64)
+    offset = 2 * 7 * 2.0 ** -24 * 255 * np.nanmax(p.vs)
+    got = host(call(p, dev_(q), G, scale)).reshape(B, G, 64).astype(np.float64)
+    for b, (want, size) in enumerate(reference(p, q, G, scale)):
+        assert np.all(np.abs(got[b] - want) <= 2.0 ** -11 * np.abs(want) + 2.0 ** -10 * size + 2.0 ** -25 + offset), b
