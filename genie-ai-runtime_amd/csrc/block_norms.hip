@@ -11,7 +11,8 @@
 // 2560 2.7 us, of which a launch is two).  fp32 from the inputs to the stores; y is formed
 // from h before h is rounded, so each output carries one rounding.  For the codes
 // 1 / sqrt(..) cancels: y / max |y| is h w / max |h w|, and that maximum is found in the same
-// pass through LDS as the sum of squares.  Loading the weights and the gate with x instead of
+// pass through LDS as the sum of squares (8191 rows of 4096, the block's output normed, 235 MB,
+// 55 us: 4.3 TB/s); only where h w leaves fp32's range does a row take a second maximum.  Loading the weights and the gate with x instead of
 // where they are used: 47.5 -> 45 us without a gate, 68.5 -> 67.6 with one, but 73 -> 102 for
 // rows of 16384 (registers) and 2.8 -> 3.0 for one row.
 #include "kq_common.h"

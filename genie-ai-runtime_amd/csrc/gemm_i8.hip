@@ -4,10 +4,13 @@
 //
 // The sums are int32 on the matrix cores and exact (K <= 131056), whatever their order;
 // the fp32 epilogue multiplies by the token's scale, then the channel's.
-// Bounds: up to 16 tokens the bytes of W (151936 x 2560 74 us, 5.3 TB/s) or, of few channels,
-// how fast a CU has them (2560 x 9728 9.5 us); to about 256 the rate at which a CU reads; beyond, the
-// matrix cores and the clock that their power leaves (8192^3 482 us, 2.28 POP/s, at 1.9 GHz,
-// of whose cycles they are busy 56 %; the rest is the waits at a stage's barrier).
+// Bounds: up to 16 tokens the bytes of W (151936 x 2560 74 us, 5.3 TB/s), but of few channels
+// its 16 a workgroup leave CUs idle (2560 x 9728 9.1 us on 160 of 256).  To about 1000 tokens the
+// waves wait, for the next stage or at its barrier (64 tokens x 6144 x 2560 8.8 us, 59 % of their
+// time; 251 x 32003 x 2064 34.5 us, 42 %).  Beyond, the matrix cores and the clock that their power leaves: 8192^3 492 us,
+// 2.23 POP/s, at 1.9 GHz, of whose cycles they are busy 57 %.  There a wave waits 47 % of its
+// time, for a stage's barrier or for its operands (a quarter's reads from LDS stand right before
+// its matrix instructions, and are waited for); which of them costs more is not measured.
 #include "gemm_i8_plan.h"
 #include "kq_common.h"
 #include "serving.h"
@@ -65,10 +68,10 @@ __device__ __forceinline__ bool packed_rows(const GemmI8Args& a) {
 // v_mfma_i32_16x16x64_i8: 16 codes of channel li / token li.  Codes go straight to registers,
 // two batches of U pieces on the way.  Waves x U:
 //   one token     151936 x 2560   19456 x 2560   6144 x 2560   2560 x 9728   1024 x 9728
-//   4 x 5             76.6            12.3           6.3           9.9           9.3
-//   4 x 8             73.8            12.2           6.4          10.7          10.1
-//   16 x 5           108              16.3           7.5           9.5           9.0
-// (us, calls one behind the other.  A workgroup for up to 64 tokens, without tiles: its own
+//   4 x 5             76.8            13.9           6.3           9.9           9.4
+//   4 x 8             74.2            13.9           6.4          10.9          10.4
+//   16 x 5           108              17.1           7.5           9.5           9.1
+// (us, calls one behind the other, W from memory.  A workgroup for up to 64 tokens, without tiles: its own
 // reading of all tokens took longer than its weights: 28 us for 2560 x 9728 against 14.)
 template <int GF_WAVES, int U>
 __global__ __launch_bounds__(64 * GF_WAVES) void gemm_i8_few_kernel(GemmI8Args a) {

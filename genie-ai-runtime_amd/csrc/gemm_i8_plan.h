@@ -18,7 +18,7 @@ constexpr int GT_K = 128;              // codes of a row in a stage of a tile
 // 14.1; 26 in one).  The plan is what these say takes least.
 // Few tokens: from 16384 channels a wave has 16 pieces on the way; from 8192 codes 16 waves
 // share K, where there is no more than a workgroup for each CU (4096 x 28672, one token 25.1 us,
-// 28.0 with four; 8192 x 9728 18.2 and 17.5).
+// 27.8 with four; with two a CU it is near: 8192 x 9728 18.3 and 19.2, 8 tokens 21.5 either way).
 enum { FEW_NONE, FEW, FEW_MANY_CHANNELS, FEW_LONG_K };
 struct GemmPlan { int few, tile, splits, whole; };
 struct TileKind { int tm, tn, share; float alone, full, tile, tiles; };

@@ -12,7 +12,7 @@
 // exponent); here a wave's keys meet NR column groups.
 //
 // Two forms.  Few columns (query heads of one KV head, of all rows): keys straight to
-// registers, four waves; 8 rows over 16384 INT8 keys of 32 / 8 heads x 128 27 us, both
+// registers, four waves; 8 rows over 16384 INT8 keys of 32 / 8 heads x 128 22 us, both
 // launches, of which the prefix's 34 MB need 6.6.  More: keys through LDS, eight waves,
 // so that up to 256 columns meet each key that is read; bound by the softmax's VALU
 // instructions beside the matrix products (64 rows of 32 / 8 heads over 32768 fp16 keys 68
@@ -47,7 +47,10 @@ PrefixPlan prefix_plan(int B, int n_heads, int n_kv, int max_prefix, int window,
     // and 17.8; INT8, 16384 keys 33.2 and 31.7: its conversions take longer with few columns)
     p.lds = cols > 64 || (cols > 32 && !int8 && span * n_kv >= 256 * 256);
     // (with a window the code for columns that do not see a key leaves no registers for two
-    // groups: 16 rows of 16 / 4 heads x 128 15.3 us)
+    // groups: 16 rows of 16 / 4 heads x 128 15.3 us.  Of fp16 keys and head_dim 128 it spills
+    // even so: 11 registers here, through LDS 4 with four row waves and 37, 52 bytes a lane,
+    // with eight.  32 / 8 heads, the last 4096 of 8192 keys and a whole prefix of 4096: 16 rows
+    // 27.0 and 22.0 us, 64 rows 41.4 and 37.0.)
     p.nr = p.lds || (cols > 16 && window == 0) ? 2 : 1;
     p.rw = p.lds ? (cols > 128 ? 8 : 4) : (cols > 16 * p.nr ? (cols > 32 * p.nr ? 4 : 2) : 1);
     const int per = 16 * p.nr * p.rw;
